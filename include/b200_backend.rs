@@ -147,6 +147,9 @@ pub mod ffi {
         pub fn rt_gather_rows(ctx: *mut RtCtx, src: *const f32, rows: i64, row_len: i64, idx: *const i32, n_idx: i64, out: *mut f32) -> RtStatus;
         pub fn rt_gather_rows_list(ctx: *mut RtCtx, n_src: c_int, srcs: *const *const f32, row_lens: *const i64, rows: i64, idx: *const i32, n_idx: i64, outs: *const *mut f32) -> RtStatus;
         pub fn rt_upload_gather_rows(ctx: *mut RtCtx, up: *mut RtUpload, n_src: c_int, srcs: *const *const f32, row_lens: *const i64, rows: i64, n_idx: i64, outs: *const *mut f32) -> RtStatus;
+        pub fn rt_embedding(ctx: *mut RtCtx, table: *const f32, rows: i64, cols: i64, ids: *const i32, n: i64, scale: f32, out: *mut f32) -> RtStatus;
+        pub fn rt_embedding_backward(ctx: *mut RtCtx, g: *const f32, ids: *const i32, n: i64, rows: i64, cols: i64, scale: f32, dtable: *mut f32, accumulate: c_int) -> RtStatus;
+        pub fn rt_token_ids(ctx: *mut RtCtx, x: *const f32, n: i64, ids: *mut i32) -> RtStatus;
         pub fn rt_sum_rows_accumulate(ctx: *mut RtCtx, x: *const f32, rows: i64, cols: i64, out: *mut f32) -> RtStatus;
         pub fn rt_reduce(ctx: *mut RtCtx, kind: c_int, x: *const f32, outer: i64, len: i64, inner: i64, out: *mut f32) -> RtStatus;
         pub fn rt_reduce_backward(ctx: *mut RtCtx, kind: c_int, x: *const f32, g: *const f32, outer: i64, len: i64, inner: i64, dx: *mut f32) -> RtStatus;
@@ -160,6 +163,8 @@ pub mod ffi {
         pub fn rt_lstm_sequence_polls(ctx: *mut RtCtx, polls: i64) -> RtStatus;
         pub fn rt_lstm_sequence(ctx: *mut RtCtx, pre: *const f32, w: *const f32, ldw: i64, h0: *const f32, c0: *const f32, steps: i64, batch: i64, hidden: i64, saved: *mut f32, h: *mut f32) -> RtStatus;
         pub fn rt_lstm_sequence_backward(ctx: *mut RtCtx, saved: *const f32, w: *const f32, ldw: i64, c0: *const f32, dh: *const f32, steps: i64, batch: i64, hidden: i64, dgates: *mut f32, dh0: *mut f32, dc0: *mut f32) -> RtStatus;
+        pub fn rt_gated_scan(ctx: *mut RtCtx, f: *const f32, v: *const f32, ld: i64, h0: *const f32, steps: i64, batch: i64, hidden: i64, h: *mut f32) -> RtStatus;
+        pub fn rt_gated_scan_backward(ctx: *mut RtCtx, f: *const f32, v: *const f32, ld: i64, h0: *const f32, h: *const f32, dh: *const f32, steps: i64, batch: i64, hidden: i64, df: *mut f32, dv: *mut f32, ldd: i64, dh0: *mut f32) -> RtStatus;
         pub fn rt_softmax_cross_entropy(ctx: *mut RtCtx, logits: *const f32, targets: *const f32, rows: i64, classes: i64, loss: *mut f32) -> RtStatus;
         pub fn rt_softmax_cross_entropy_backward(ctx: *mut RtCtx, logits: *const f32, targets: *const f32, g: *const f32, rows: i64, classes: i64, dlogits: *mut f32, dtargets: *mut f32) -> RtStatus;
         pub fn rt_softmax_nll_scaled(ctx: *mut RtCtx, logits: *const f32, targets: *const f32, rows: i64, classes: i64, scale: f32, divisor: f32, loss: *mut f32) -> RtStatus;
@@ -190,6 +195,8 @@ pub mod ffi {
         pub fn rt_adagrad_step(ctx: *mut RtCtx, param: *mut f32, grad: *const f32, accum: *mut f32, n: i64, lr: f32, epsilon: f32) -> RtStatus;
         pub fn rt_adam_step(ctx: *mut RtCtx, param: *mut f32, grad: *const f32, m: *mut f32, v: *mut f32, n: i64, lr: f32, beta1: f32, beta2: f32, epsilon: f32, t: i64) -> RtStatus;
         pub fn rt_optimizer_step_multi(ctx: *mut RtCtx, kind: c_int, n_tensors: c_int, params: *const *mut f32, grads: *const *const f32, state1: *const *mut f32, state2: *const *mut f32, sizes: *const i64, lr: f32, beta1: f32, beta2: f32, epsilon: f32, momentum: f32, t: i64, grad_scale: f32, clip: c_int, clip_lo: f32, clip_hi: f32) -> RtStatus;
+        pub fn rt_muon_step_multi(ctx: *mut RtCtx, n_tensors: c_int, params: *const *mut f32, grads: *const *const f32, momenta: *const *mut f32, rows: *const i64, cols: *const i64, lr: f32, momentum: f32, nesterov: c_int, weight_decay: f32, steps: c_int, grad_scale: f32) -> RtStatus;
+        pub fn rt_orthogonalize_list(ctx: *mut RtCtx, count: c_int, xs: *const *const f32, rows: *const i64, cols: *const i64, steps: c_int, outs: *const *mut f32) -> RtStatus;
         pub fn rt_pack_flat(ctx: *mut RtCtx, n_tensors: c_int, srcs: *const *const f32, sizes: *const i64, flat: *mut f32, clip: c_int, clip_lo: f32, clip_hi: f32) -> RtStatus;
         pub fn rt_dp_unique_id(id: *mut u8) -> RtStatus;
         pub fn rt_dp_init(ctx: *mut RtCtx, rank: c_int, world: c_int, id: *const u8) -> RtStatus;

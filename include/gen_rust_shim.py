@@ -21,7 +21,7 @@ C2RUST = {
     "rt_ctx*": "*mut RtCtx", "rt_ctx**": "*mut *mut RtCtx", "rt_graph*": "*mut RtGraph", "rt_graph**": "*mut *mut RtGraph",
     "rt_upload*": "*mut RtUpload", "rt_upload**": "*mut *mut RtUpload", "rt_event*": "*mut RtEvent", "rt_event**": "*mut *mut RtEvent",
     "int": "c_int", "int*": "*mut c_int", "const int*": "*const c_int", "int* const*": "*const *mut c_int",
-    "int32_t": "i32", "const int32_t*": "*const i32", "int64_t": "i64", "int64_t*": "*mut i64", "const int64_t*": "*const i64",
+    "int32_t": "i32", "int32_t*": "*mut i32", "const int32_t*": "*const i32", "int64_t": "i64", "int64_t*": "*mut i64", "const int64_t*": "*const i64",
     "uint32_t": "u32", "uint64_t": "u64", "uint64_t*": "*mut u64", "size_t": "usize", "float": "f32", "float*": "*mut f32", "const float*": "*const f32",
     "double*": "*mut f64", "float* const*": "*const *mut f32", "const float* const*": "*const *const f32",
     "void*": "*mut c_void", "void**": "*mut *mut c_void", "const void*": "*const c_void", "void* const*": "*const *mut c_void",

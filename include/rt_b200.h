@@ -286,6 +286,18 @@ rt_status rt_gather_rows_list(rt_ctx* ctx, int n_src, const float* const* srcs, 
 rt_status rt_upload_gather_rows(rt_ctx* ctx, rt_upload* up, int n_src, const float* const* srcs, const int64_t* row_lens, int64_t rows,
                                 int64_t n_idx, float* const* outs);
 
+/* ---- token embeddings (no counterpart in the reference, whose char-LSTM example multiplies one-hot rows with its weights:
+ * examples/lstm_char_rnn_cpu.rs) --------------------------------------------------------------------------------------
+ * ids: n int32 row numbers in DEVICE memory; one outside [0, rows) is padding.
+ * out[i, :] = scale * table[ids[i], :] for a row-major table[rows, cols]; zeros where ids[i] is padding. */
+rt_status rt_embedding(rt_ctx* ctx, const float* table, int64_t rows, int64_t cols, const int32_t* ids, int64_t n, float scale, float* out);
+/* dtable[r, :] = scale * the sum of g[i, :] over the i with ids[i] = r, which are added in a fixed order: the same inputs give the same bits.
+ * With accumulate != 0 it is added to what is there, and rows without a token are neither read nor written. */
+rt_status rt_embedding_backward(rt_ctx* ctx, const float* g, const int32_t* ids, int64_t n, int64_t rows, int64_t cols, float scale, float* dtable,
+                                int accumulate);
+/* ids[i] = x[i], which holds whole numbers as floats like the results of argmax; -1 for a fraction, NaN and what int32 does not hold. */
+rt_status rt_token_ids(rt_ctx* ctx, const float* x, int64_t n, int32_t* ids);
+
 /* out[c] += sum over r of x[r, c] for a row-major x[rows, cols]: the gradient of a bias that already holds a gradient (a bias
  * used at every timestep of a recurrent layer), accumulated in place in one launch.  Eight row lanes per column: meant for few rows. */
 rt_status rt_sum_rows_accumulate(rt_ctx* ctx, const float* x, int64_t rows, int64_t cols, float* out);
@@ -334,6 +346,15 @@ rt_status rt_lstm_sequence(rt_ctx* ctx, const float* pre, const float* w, int64_
                            int64_t batch, int64_t hidden, float* saved, float* h);
 rt_status rt_lstm_sequence_backward(rt_ctx* ctx, const float* saved, const float* w, int64_t ldw, const float* c0, const float* dh, int64_t steps,
                                     int64_t batch, int64_t hidden, float* dgates, float* dh0, float* dc0);
+
+/* Gated linear recurrence over a sequence, time-major (no counterpart in the reference): a_t = sigmoid(f_t), h_t = a_t h_{t-1} + (1 - a_t) v_t.
+ * f, v: [steps*batch, hidden] with rows ld floats apart: two matrices, or two column blocks of one.  h0 [batch, hidden] or NULL for zeros;
+ * h [steps*batch, hidden]; with one timestep h may be h0 (the state of a model that generates, updated in place).  f = +inf keeps the state
+ * (padding at a sequence's end), f = -inf takes v alone (a sequence's first timestep among others), if state and v are finite.
+ * Backward, from h and dh = the gradient of every h_t: df, dv with rows ldd apart, dh0 [batch, hidden] or NULL. */
+rt_status rt_gated_scan(rt_ctx* ctx, const float* f, const float* v, int64_t ld, const float* h0, int64_t steps, int64_t batch, int64_t hidden, float* h);
+rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, int64_t ld, const float* h0, const float* h, const float* dh, int64_t steps,
+                                 int64_t batch, int64_t hidden, float* df, float* dv, int64_t ldd, float* dh0);
 
 /* Fused classification loss (no counterpart in the reference, whose examples spell the chain out:
  * examples/train_mnist_cpu.rs:63-97): loss[0] = -(1/rows) * sum over rows and classes of targets * log_softmax(logits).
@@ -463,6 +484,16 @@ rt_status rt_optimizer_step_multi(rt_ctx* ctx, int kind, int n_tensors, float* c
                                   const int64_t* sizes, float lr, float beta1, float beta2, float epsilon,
                                   float momentum, int64_t t, float grad_scale, int clip, float clip_lo,
                                   float clip_hi);
+
+/* Muon (no counterpart in the reference): momentum whose singular values are brought near one before it is applied, for matrices
+ * [rows, cols] that rows are multiplied with (x * W).  Per matrix: m = momentum * m + s * g with s = grad_scale; u = m, or s * g + momentum * m
+ * with nesterov; p = (1 - lr * weight_decay) * p - lr * sqrt(max(1, cols / rows)) * O(u).  O(u): `steps` (0 .. 64; five are usual) times
+ * X = (a I + b G + c G^2) X, G = X X^T on the shorter side, from X = u / (|u| + 1e-7), with a, b, c = 3.4445, -4.7750, 2.0315.  Products
+ * to about fp32's precision.  All matrices of the list are worked on together.  Parameters and momenta must not overlap. */
+rt_status rt_muon_step_multi(rt_ctx* ctx, int n_tensors, float* const* params, const float* const* grads, float* const* momenta, const int64_t* rows,
+                             const int64_t* cols, float lr, float momentum, int nesterov, float weight_decay, int steps, float grad_scale);
+/* outs[i] = O(xs[i]) alone; outs[i] may be xs[i]. */
+rt_status rt_orthogonalize_list(rt_ctx* ctx, int count, const float* const* xs, const int64_t* rows, const int64_t* cols, int steps, float* const* outs);
 
 /* ---- data-parallel gradient exchange (no counterpart in the reference: it has no distributed code) */
 /* Copies a list of gradient tensors into one flat buffer (optionally clamping), so that one

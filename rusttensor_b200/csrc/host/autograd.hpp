@@ -100,7 +100,8 @@ struct OpType {
     Sigmoid, Sqrt, Tanh, Softplus, Max, Min, Prod, LogSumExp, ArgMax, ArgMin, Powf, Square,
     Maximum, Minimum, Elu, Transpose, Sin, Cos, Tan, Conv2d, MaxPool2D, Conv2DTranspose, Slice,
     Concat, ExpandDims, Squeeze, Clip, DivScalar, MulScalar,
-    FusedReluMaxPool2D, FusedSoftmaxNll, FusedLstmCellC, FusedLstmCellH, FusedConvReluMaxPool2D, FusedLstmSequence  // fused forward ops added beside the reference's (ops::fused_*)
+    FusedReluMaxPool2D, FusedSoftmaxNll, FusedLstmCellC, FusedLstmCellH, FusedConvReluMaxPool2D, FusedLstmSequence,  // fused forward ops added beside the reference's (ops::fused_*)
+    Embedding, GatedScan                        // ops that the reference does not have
   } kind;
   std::optional<size_t> axis;          // Mean/Sum/Max/Min/Prod/LogSumExp(Option), LogSoftmax/ArgMax/...
   float scalar = 0.f;                  // Elu(alpha), MulScalar, DivScalar
@@ -120,7 +121,7 @@ struct OpType {
       "Div", "Exp", "Ln", "Broadcast", "View", "Abs", "Sigmoid", "Sqrt", "Tanh", "Softplus", "Max",
       "Min", "Prod", "LogSumExp", "ArgMax", "ArgMin", "Powf", "Square", "Maximum", "Minimum", "Elu",
       "Transpose", "Sin", "Cos", "Tan", "Conv2d", "MaxPool2D", "Conv2DTranspose", "Slice", "Concat",
-      "ExpandDims", "Squeeze", "Clip", "DivScalar", "MulScalar", "FusedReluMaxPool2D", "FusedSoftmaxNll", "FusedLstmCellC", "FusedLstmCellH", "FusedConvReluMaxPool2D", "FusedLstmSequence"};
+      "ExpandDims", "Squeeze", "Clip", "DivScalar", "MulScalar", "FusedReluMaxPool2D", "FusedSoftmaxNll", "FusedLstmCellC", "FusedLstmCellH", "FusedConvReluMaxPool2D", "FusedLstmSequence", "Embedding", "GatedScan"};
     return n[(int)kind];
   }
 };
@@ -1084,6 +1085,68 @@ Tensor<B> fused_lstm_sequence(const Tensor<B>& x, const Tensor<B>& w, const Tens
   }
 }
 
+// ---- ops that the reference does not have ---------------------------------------------------------------------------------
+// scale * table[ids], a row for every entry of ids, which holds whole numbers like the results of argmax: [ids' shape..., cols].  What is no
+// row's number is padding: zeros, and no gradient.  A backend without the kernels multiplies one-hot rows with the table, as the
+// reference's char-LSTM example does (examples/lstm_char_rnn_cpu.rs).
+template <class B>
+Tensor<B> embedding(const Tensor<B>& table, const Tensor<B>& ids, float scale) {
+  const Shape ts = table.shape(), is = ids.shape();
+  if (ts.size() != 2) throw Error::invalid_op("embedding expects a table [rows, cols]");
+  Shape os = is;
+  os.push_back(ts[1]);
+  if constexpr (!HasFusedForward<B>::value) {
+    const std::vector<float> at = ids.to_vec();
+    std::vector<float> hot(at.size() * ts[0], 0.f);
+    for (size_t i = 0; i < at.size(); ++i)
+      for (size_t r = 0; r < ts[0]; ++r)
+        if (at[i] == (float)r) hot[i * ts[0] + r] = 1.f;
+    return view(mul_scalar(matmul(Tensor<B>::from_vec(std::move(hot), Shape{at.size(), ts[0]}, false), table), scale), os);
+  } else {
+    St<B> numbers = B::token_ids(ids.data());  // kept for the gradient
+    Tensor<B> t(B::embedding(table.data(), numbers, os, scale), table.requires_grad());
+    if (table.requires_grad()) {
+      OpType ot(OpType::Embedding);
+      ot.scalar = scale;
+      t.set_op(Op<B>(ot, {table, ids}, [numbers](const Op<B>& op, const St<B>& g) {
+        const Shape of_ids = op.inputs[1].shape();
+        return Grads<B>{B::embedding_backward(op, numbers, g), op.inputs[1].requires_grad() ? B::zeros(of_ids) : B::unused_grad(of_ids)};
+      }));
+    }
+    return t;
+  }
+}
+
+// A gated linear recurrence over a time-major sequence of `steps` timesteps: gates [steps * batch, 2H] with the column blocks f and v,
+// h_t = a h_{t-1} + (1 - a) v_t with a = sigmoid(f_t), from h0 [batch, H] or zeros; all states [steps * batch, H].
+template <class B>
+Tensor<B> gated_scan(const Tensor<B>& gates, const Tensor<B>* h0, size_t steps) {
+  const Shape gs = gates.shape();
+  if (gs.size() != 2 || steps == 0 || gs[0] == 0 || gs[0] % steps != 0) throw Error::invalid_op("gated_scan expects time-major gates [steps * batch, 2 * hidden]");
+  const size_t Bn = gs[0] / steps, H = gs[1] / 2;
+  if (H == 0 || gs[1] != 2 * H) throw Error::invalid_op("gated_scan expects two columns of gates for each hidden unit");
+  if (h0 && h0->shape() != Shape{Bn, H}) throw Error::incompatible("gated_scan", gs, h0->shape());
+  if constexpr (!HasFusedForward<B>::value) {
+    Tensor<B> h = h0 ? *h0 : Tensor<B>::zeros({Bn, H}, false);
+    std::vector<Tensor<B>> hs;
+    for (size_t t = 0; t < steps; ++t) {
+      Tensor<B> f = slice(gates, {{t * Bn, (t + 1) * Bn}, {0, H}}), v = slice(gates, {{t * Bn, (t + 1) * Bn}, {H, 2 * H}});
+      h = add(mul(sigmoid(f), h), mul(sigmoid(mul_scalar(f, -1.f)), v));
+      hs.push_back(h);
+    }
+    return concat<B>(hs, 0);
+  } else {
+    Tensor<B> t(B::gated_scan(gates.data(), h0 ? &h0->data() : nullptr, steps), gates.requires_grad() || (h0 && h0->requires_grad()));
+    if (t.requires_grad()) {
+      std::vector<Tensor<B>> in{gates};
+      if (h0) in.push_back(*h0);
+      t.set_op(Op<B>(OpType(OpType::GatedScan), in, [steps](const Op<B>& op, const St<B>& g) { return B::gated_scan_backward(op, g, steps); }));
+      t.inner->op->cached_outputs = t.data();
+    }
+    return t;
+  }
+}
+
 }  // namespace ops
 
 template <class B>
@@ -1249,6 +1312,62 @@ struct AdaGrad {
                       epsilon);
   }
   void zero_grad() { zero_grad_all(parameters); }
+};
+
+// Muon (not in the reference): momentum with its singular values brought near one, for matrices; rt_muon_step_multi says what it computes.
+// A backend without that step runs it product by product.
+template <class B>
+struct Muon {
+  std::vector<Tensor<B>> parameters;
+  float learning_rate, momentum, weight_decay;
+  bool nesterov;
+  int ns_steps;
+  std::vector<typename B::Storage> momenta;
+  Muon(std::vector<Tensor<B>> p, float lr, float mu, bool nest, float wd, int steps)
+      : parameters(std::move(p)), learning_rate(lr), momentum(mu), weight_decay(wd), nesterov(nest), ns_steps(steps) {
+    if (steps < 0 || steps > 64) throw Error::invalid_op("Muon takes between 0 and 64 steps");
+    for (auto& x : parameters) {
+      if (x.shape().size() != 2) throw Error::invalid_op("Muon takes matrices: give other parameters to another optimizer");
+      momenta.push_back(B::zeros(x.shape()));
+    }
+  }
+  void step() {
+    if constexpr (KeepsOutputs<B>::value) {
+      std::vector<typename B::Storage*> p, m;
+      std::vector<typename B::Storage> g;
+      for (auto& u : collect_updates(parameters)) {
+        p.push_back(&parameters[u.first].data_mut());
+        g.push_back(u.second);
+        m.push_back(&momenta[u.first]);
+      }
+      B::muon_step_all(p, g, m, learning_rate, momentum, nesterov, weight_decay, ns_steps);
+    } else {
+      for (auto& u : collect_updates(parameters)) step_one(parameters[u.first].data_mut(), u.second, momenta[u.first]);
+    }
+  }
+  void zero_grad() { zero_grad_all(parameters); }
+
+ private:
+  using S = typename B::Storage;
+  void step_one(S& p, const S& g, S& m) const {
+    const Shape s = B::shape(p);
+    if (s[0] == 0 || s[1] == 0) return;
+    m = B::add(B::mul_scalar(m, momentum), g);
+    S x = nesterov ? B::add(g, B::mul_scalar(m, momentum)) : m;
+    double squares = 0.0;
+    for (float v : B::copy_to_host(x)) squares += (double)v * v;
+    x = B::mul_scalar(x, (float)(1.0 / (std::sqrt(squares) + 1e-7)));
+    const bool tall = s[0] > s[1];
+    if (tall) x = B::transpose(x);
+    for (int k = 0; k < ns_steps; ++k) {
+      S gram = B::matmul(x, B::transpose(x));
+      S poly = B::add(B::mul_scalar(gram, -4.7750f), B::mul_scalar(B::matmul(gram, gram), 2.0315f));
+      x = B::add(B::mul_scalar(x, 3.4445f), B::matmul(poly, x));
+    }
+    if (tall) x = B::transpose(x);
+    const float by = (float)(learning_rate * std::sqrt(std::max(1.0, (double)s[1] / (double)s[0])));
+    p = B::sub(B::mul_scalar(p, 1.f - learning_rate * weight_decay), B::mul_scalar(x, by));
+  }
 };
 
 }  // namespace optim

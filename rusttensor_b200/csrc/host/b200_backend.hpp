@@ -1424,6 +1424,59 @@ struct B200Backend {
     return out;
   }
 
+  // ---- token embeddings, gated linear recurrence ----------------------------------------------------------------------------------
+  // The numbers as int32, in a buffer of the same size.
+  static Storage token_ids(const Storage& x) {
+    const float* p = x.ptr();
+    Storage ids = alloc(x.shape);
+    check(rt_token_ids(ctx(), p, (int64_t)x.numel(), reinterpret_cast<int32_t*>(ids.ptr())));
+    return ids;
+  }
+  static Storage embedding(const Storage& table, const Storage& ids, const Shape& shape, float scale) {
+    const float* p = table.ptr();
+    Storage out = alloc(shape);
+    check(rt_embedding(ctx(), p, (int64_t)table.shape[0], (int64_t)table.shape[1], reinterpret_cast<const int32_t*>(ids.ptr()), (int64_t)ids.numel(), scale,
+                       out.ptr()));
+    return out;
+  }
+  static Storage embedding_backward(const OpB& o, const Storage& ids, const Storage& g) {
+    const Shape ts = o.inputs[0].shape();
+    Shape want = ids.shape;
+    want.push_back(ts[1]);
+    if (g.shape != want) throw Error::shape_mismatch(want, g.shape);
+    const float* pg = g.ptr();
+    Storage d = alloc(ts);
+    check(rt_embedding_backward(ctx(), pg, reinterpret_cast<const int32_t*>(ids.ptr()), (int64_t)ids.numel(), (int64_t)ts[0], (int64_t)ts[1], o.op_type.scalar,
+                                d.ptr(), 0));
+    return d;
+  }
+  static Storage gated_scan(const Storage& gates, const Storage* h0, size_t steps) {
+    const int64_t rows = (int64_t)gates.shape[0], H = (int64_t)gates.shape[1] / 2;
+    const float *p = gates.ptr(), *p0 = h0 ? h0->ptr() : nullptr;
+    Storage h = alloc({gates.shape[0], (size_t)H});
+    check(rt_gated_scan(ctx(), p, p + H, 2 * H, p0, (int64_t)steps, rows / (int64_t)steps, H, h.ptr()));
+    return h;
+  }
+  static std::vector<Storage> gated_scan_backward(const OpB& o, const Storage& g, size_t steps) {
+    const Storage &gates = o.inputs[0].data(), &h = *o.cached_outputs;
+    if (g.shape != h.shape) throw Error::shape_mismatch(h.shape, g.shape);
+    const int64_t rows = (int64_t)gates.shape[0], H = (int64_t)gates.shape[1] / 2, batch = rows / (int64_t)steps;
+    const bool given = o.inputs.size() > 1;
+    const float *p = gates.ptr(), *p0 = given ? o.inputs[1].data().ptr() : nullptr, *pg = g.ptr(), *states = h.ptr();
+    const bool written = h.buf->escaped && !lazy::capturing();  // perhaps, since
+    lazy::Block again(ctx(), written ? (size_t)(rows * H) : 1);
+    if (written) {
+      check(rt_gated_scan(ctx(), p, p + H, 2 * H, p0, (int64_t)steps, batch, H, again.ptr));
+      states = again.ptr;
+    }
+    const bool to_start = given && o.inputs[1].requires_grad();
+    std::vector<Storage> out{alloc(gates.shape)};
+    if (given) out.push_back(to_start ? alloc(o.inputs[1].shape()) : unused_grad(o.inputs[1].shape()));
+    float* d = out[0].ptr();
+    check(rt_gated_scan_backward(ctx(), p, p + H, 2 * H, p0, states, pg, (int64_t)steps, batch, H, d, d + H, 2 * H, to_start ? out[1].ptr() : nullptr));
+    return out;
+  }
+
   // ---- sequences on the tape (Tensor::backward) ----------------------------------------------------------------------------------
   // An LSTM that was written op by op and computed as one (lazy::rewrite_recurrence) goes backward as one, too: its nodes take no part in the
   // walk, and once everything else is done the gradients of all its states go through rt_lstm_sequence_backward.  Its weights and bias are
@@ -1613,6 +1666,32 @@ struct B200Backend {
         b.push_back(nullptr);
       }
       n.push_back((int64_t)ps[i]->numel());
+    }
+    launch();
+  }
+
+  // A step of Muon for all matrices together.
+  static void muon_step_all(const std::vector<Storage*>& ps, const std::vector<Storage>& gs, const std::vector<Storage*>& ms, float lr, float momentum,
+                            bool nesterov, float weight_decay, int steps) {
+    std::vector<float*> p, m;
+    std::vector<const float*> g;
+    std::vector<int64_t> rows, cols;
+    auto launch = [&] {
+      if (!p.empty())
+        check(rt_muon_step_multi(ctx(), (int)p.size(), p.data(), g.data(), m.data(), rows.data(), cols.data(), lr, momentum, nesterov, weight_decay, steps, 1.f));
+      p.clear(); m.clear(); g.clear(); rows.clear(); cols.clear();
+    };
+    for (size_t i = 0; i < ps.size(); ++i) {
+      if (ps[i]->numel() == 0) continue;
+      const float* pg = gs[i].ptr();
+      if (std::find(p.begin(), p.end(), ps[i]->buf->ptr) != p.end()) launch();  // a parameter listed twice is updated twice, in order
+      make_unique(*ps[i]);
+      make_unique(*ms[i]);
+      p.push_back(ps[i]->ptr());
+      g.push_back(pg);
+      m.push_back(ms[i]->ptr());
+      rows.push_back((int64_t)ps[i]->shape[0]);
+      cols.push_back((int64_t)ps[i]->shape[1]);
     }
     launch();
   }

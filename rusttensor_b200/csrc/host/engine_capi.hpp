@@ -27,11 +27,12 @@ struct Registry {
   std::map<int64_t, Tensor<B>> tensors;
   std::map<int64_t, std::shared_ptr<models::Trainer<B>>> trainers;
   struct Optim {
-    int kind;  // 0 sgd 1 adam 2 momentum 3 adagrad
+    int kind;  // 0 sgd 1 adam 2 momentum 3 adagrad 4 muon
     std::shared_ptr<optim::Sgd<B>> sgd;
     std::shared_ptr<optim::Adam<B>> adam;
     std::shared_ptr<optim::MomentumSGD<B>> mom;
     std::shared_ptr<optim::AdaGrad<B>> ada;
+    std::shared_ptr<optim::Muon<B>> muon;
   };
   std::map<int64_t, Optim> optims;
   int64_t next = 1;
@@ -67,6 +68,7 @@ inline std::optional<size_t> opt_axis(int64_t a) {
 //   max_pool2d: ip = kh,kw,sh,sw,ph,pw       view/broadcast_to: ip = shape
 //   elu/mul_scalar/div_scalar/powf_scalar: fp[0] ; clip: fp[0],fp[1]
 //   mse_loss/bce_with_logits: ip[0] = reduction (0 none,1 sum,2 mean) ; softmax_cross_entropy: ip = axis,reduction
+//   embedding: inputs = table,ids ; fp[0] = scale       gated_scan: inputs = gates[,h0] ; ip[0] = steps
 template <class B>
 Tensor<B> run_op(const std::string& name, const std::vector<Tensor<B>>& in, const std::vector<int64_t>& ip,
                  const std::vector<double>& fp) {
@@ -150,6 +152,12 @@ Tensor<B> run_op(const std::string& name, const std::vector<Tensor<B>>& in, cons
   if (name == "softmax_cross_entropy") {
     need(2);
     return ops::softmax_cross_entropy(in[0], in[1], (size_t)ipa(0), red(ipa(1)));
+  }
+  if (name == "embedding") { need(2); return ops::embedding(in[0], in[1], fpa(0)); }
+  if (name == "gated_scan") {
+    if (in.size() != 1 && in.size() != 2) throw Error::invalid_op(name + ": expected 1 or 2 inputs");
+    if (ipa(0) < 1) throw Error::invalid_op(name + ": expected one timestep or more");
+    return ops::gated_scan(in[0], in.size() == 2 ? &in[1] : nullptr, (size_t)ipa(0));
   }
   throw Error::invalid_op("unknown op '" + name + "'");
 }
@@ -261,7 +269,8 @@ int guarded(F f) {
       for (size_t i = 0; i < grads.size(); ++i) outs[i] = r.put(rt::Tensor<BK>(std::move(grads[i]), false));  \
     });                                                                                                       \
   }                                                                                                           \
-  /* optimizers: kind 0 Sgd(lr) 1 Adam(lr,b1,b2,eps) 2 MomentumSGD(lr,mu) 3 AdaGrad(lr,eps) */                \
+  /* optimizers: kind 0 Sgd(lr) 1 Adam(lr,b1,b2,eps) 2 MomentumSGD(lr,mu) 3 AdaGrad(lr,eps)                   \
+     4 Muon(lr,mu,nesterov,weight_decay,steps) */                                                             \
   int P##_optim_create(int kind, const int64_t* params, int n, const double* hp, int n_hp, int64_t* out) {    \
     return rt::capi::guarded<BK>([&](auto& r) {                                                               \
       std::vector<rt::Tensor<BK>> ps;                                                                         \
@@ -276,6 +285,8 @@ int guarded(F f) {
       else if (kind == 1) o.adam = std::make_shared<rt::optim::Adam<BK>>(ps, hpa(0), hpa(1), hpa(2), hpa(3)); \
       else if (kind == 2) o.mom = std::make_shared<rt::optim::MomentumSGD<BK>>(ps, hpa(0), hpa(1));           \
       else if (kind == 3) o.ada = std::make_shared<rt::optim::AdaGrad<BK>>(ps, hpa(0), hpa(1));               \
+      else if (kind == 4)                                                                                     \
+        o.muon = std::make_shared<rt::optim::Muon<BK>>(ps, hpa(0), hpa(1), hpa(2) != 0.f, hpa(3), (int)hpa(4));\
       else throw rt::Error::invalid_op("optim_create: unknown kind");                                         \
       r.optims[r.next] = o;                                                                                   \
       *out = r.next++;                                                                                        \
@@ -288,6 +299,7 @@ int guarded(F f) {
       if (o.adam) o.adam->step();                                                                             \
       if (o.mom) o.mom->step();                                                                               \
       if (o.ada) o.ada->step();                                                                               \
+      if (o.muon) o.muon->step();                                                                             \
     });                                                                                                       \
   }                                                                                                           \
   int P##_optim_zero_grad(int64_t h) {                                                                        \
@@ -297,6 +309,7 @@ int guarded(F f) {
       if (o.adam) o.adam->zero_grad();                                                                        \
       if (o.mom) rt::optim::zero_grad_all(o.mom->parameters);                                                 \
       if (o.ada) o.ada->zero_grad();                                                                          \
+      if (o.muon) o.muon->zero_grad();                                                                        \
     });                                                                                                       \
   }                                                                                                           \
   /* which: 0 = first state (m / velocity / accumulator), 1 = second state (v) */                             \
@@ -306,6 +319,7 @@ int guarded(F f) {
       if (o.adam) *out = r.put(rt::Tensor<BK>(which == 0 ? o.adam->m_states.at(idx) : o.adam->v_states.at(idx), false)); \
       else if (o.mom) *out = r.put(rt::Tensor<BK>(o.mom->velocities.at(idx), false));                         \
       else if (o.ada) *out = r.put(rt::Tensor<BK>(o.ada->accumulated_sq_grad.at(idx), false));                \
+      else if (o.muon) *out = r.put(rt::Tensor<BK>(o.muon->momenta.at(idx), false));                          \
       else throw rt::Error::invalid_op("optim_state: optimizer has no state");                                \
     });                                                                                                       \
   }                                                                                                           \

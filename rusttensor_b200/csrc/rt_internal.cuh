@@ -191,6 +191,20 @@ static inline void rt_launch(rt_ctx* ctx, void (*kern)(Params...), dim3 grid, di
   cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);  // errors: RT_LAUNCHED
 }
 
+// Makes the context's device the current one while it lives: a caller's thread may be at another.
+struct RtOnDevice {
+  int before = -1;
+  explicit RtOnDevice(const rt_ctx* ctx) {
+    int now = ctx->device;
+    if (cudaGetDevice(&now) == cudaSuccess && now != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = now;
+  }
+  ~RtOnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+  RtOnDevice(const RtOnDevice&) = delete;
+  RtOnDevice& operator=(const RtOnDevice&) = delete;
+};
+
 static inline int rt_grid_for(rt_ctx* ctx, int64_t work_items, int per_block, int max_waves = 8) {
   int64_t blocks = (work_items + per_block - 1) / per_block;
   int64_t cap = (int64_t)ctx->sm_count * max_waves;

@@ -160,6 +160,9 @@ _Ops.binary_cross_entropy_with_logits = lambda self, l, t, reduction="mean": sel
     "binary_cross_entropy_with_logits", [l, t], [_RED[reduction]])
 _Ops.softmax_cross_entropy = lambda self, l, t, axis, reduction="mean": self._run(
     "softmax_cross_entropy", [l, t], [int(axis), _RED[reduction]])
+# not in the reference: rows of a table by number (whole numbers in a tensor, as argmax gives them), and a gated linear recurrence
+_Ops.embedding = lambda self, table, ids, scale=1.0: self._run("embedding", [table, ids], (), [scale])
+_Ops.gated_scan = lambda self, gates, steps, h0=None: self._run("gated_scan", [gates] + ([h0] if h0 is not None else []), [int(steps)])
 
 
 class Optimizer:
@@ -336,6 +339,10 @@ class Engine:
 
     def AdaGrad(self, params, lr, epsilon=1e-8):
         return Optimizer(self, 3, params, [lr, epsilon])
+
+    def Muon(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5):
+        """Momentum with its singular values brought near one, for parameters that are matrices (not in the reference)."""
+        return Optimizer(self, 4, params, [lr, momentum, 1.0 if nesterov else 0.0, weight_decay, ns_steps])
 
     def trainer(self, config, dims):
         return Trainer(self, config, dims)
