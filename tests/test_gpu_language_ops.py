@@ -60,7 +60,7 @@ def test_embedding(capi, rows, cols, n, shift):
 
 
 @pytest.mark.parametrize("accumulate", [0, 1])
-@pytest.mark.parametrize("rows,cols,n", TABLES + [(65, 512, 8192), (5, 36, 20000), (40000, 20, 70000), (300, 8, 140001)])
+@pytest.mark.parametrize("rows,cols,n", TABLES + [(65, 512, 8192), (900, 132, 128), (900, 132, 129), (2, 300, 127), (5, 36, 20000), (40000, 20, 70000), (300, 8, 140001)])
 def test_embedding_backward(capi, rows, cols, n, accumulate):
     r = rng(rows + cols + n)
     g, ids, old = r.standard_normal((n, cols)).astype(np.float32), tokens(r, rows, n), r.standard_normal((rows, cols)).astype(np.float32)
@@ -77,10 +77,11 @@ def test_embedding_backward(capi, rows, cols, n, accumulate):
     assert np.array_equal(got[untouched], old[untouched] if accumulate else np.zeros_like(old[untouched]))
 
 
-def test_embedding_backward_of_one_token_only(capi):
+@pytest.mark.parametrize("count", [1, 33, 100, 3000, 70001])
+def test_embedding_backward_of_one_token_only(capi, count):
     """All tokens the same, all of them padding, and rows of infinities and NaN that are padding."""
     r = rng(8)
-    n, rows, cols = 3000, 40, 68
+    n, rows, cols = int(count), 40, 68
     g = r.standard_normal((n, cols)).astype(np.float32)
     for ids in (np.full(n, 39), np.full(n, 0), np.full(n, -5), np.full(n, 40)):
         bad = g.copy()
@@ -90,6 +91,23 @@ def test_embedding_backward_of_one_token_only(capi):
         d, dg, di = capi.to_device(r.standard_normal((rows, cols))), capi.to_device(bad), device_ids(capi, ids)
         capi.call("embedding_backward", dg.ptr, di.ptr, i64(n), i64(rows), i64(cols), f32(1.0), d.ptr, 0)
         assert within(d.numpy(), want, bound)
+
+
+@pytest.mark.parametrize("n", [60, 4000])
+def test_embedding_backward_special_values(capi, n):
+    """Infinities and NaN of a position go to its token's row and nowhere else, and rows without a token are zero whatever the scale is."""
+    r = rng(n)
+    rows, cols = 50, 20
+    g, ids = r.standard_normal((n, cols)).astype(np.float32), r.integers(0, rows - 9, n)
+    g[7, 3], g[11, 4] = np.nan, np.inf
+    d, dg, di = capi.to_device(np.full((rows, cols), 3.0)), capi.to_device(g), device_ids(capi, ids)
+    capi.call("embedding_backward", dg.ptr, di.ptr, i64(n), i64(rows), i64(cols), f32(2.0), d.ptr, 0)
+    got = d.numpy()
+    bad = np.zeros((rows, cols), bool)
+    bad[ids[7], 3] = bad[ids[11], 4] = True
+    assert np.isnan(got[ids[7], 3]) and np.isinf(got[ids[11], 4]) and np.isfinite(got[~bad]).all()
+    capi.call("embedding_backward", dg.ptr, di.ptr, i64(n), i64(rows), i64(cols), f32(np.inf), d.ptr, 0)
+    assert np.all(d.numpy()[rows - 9 :] == 0)
 
 
 def test_embedding_scale_and_special_values(capi):
