@@ -5,9 +5,25 @@
 //
 // No gate depends on the state, so nothing but the state itself goes from timestep to timestep.  f = +inf keeps the state (a padded
 // timestep), f = -inf forgets it (the first one of another sequence), both without a gradient.
+//
+// Timesteps in a row are one timestep: from state h they lead to A h + B, with A the product of the gates.  So the sequence is walked through in
+// stretches.  The threads have some columns and timesteps each, units of lanes, warps and the blocks of a cluster one stretch after
+// the other; they tell one another their A and B (shuffles, shared memory, the cluster's), after which every thread knows the state
+// that it starts from and all of its outputs are a multiply-add each.  Everything is read and written once; the loads of the next stretch
+// are in flight meanwhile, or those of other blocks.  What is added in which order depends on the sizes alone.
+//
+// Bound by memory, 12 bytes an element forward and 24 backward, and near that by the instructions (about 40 and 60 an element; 88 backward
+// with one column at a time).  Measured, in TB/s of those bytes: 128 timesteps of 64 x 512 11.7 us forward (4.3), 19.5 backward (5.2); 1000 of
+// 16 x 1000 38.3 (5.0); 65536 of 1 x 512 83.8 (4.8) and 163 (4.9); 30011 of 3 x 257 backward 156 (3.6).  A thread per column, which reads ahead
+// eight timesteps, takes 24 us for the first and 9.4 ms for the third; it remains for up to eight timesteps.
+#include <cooperative_groups.h>
+
 #include "rt_internal.cuh"
+#include "tc_common.cuh"
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kThreads = 128, kAhead = 8;
 
@@ -21,10 +37,15 @@ struct ScanArgs {
   float *df, *dv;
   int64_t ldd;
   float* dh0;
+  int* status;
 };
-// sigmoid(f) and 1 - sigmoid(f), each to the last bits: the smaller one is not the difference of two near ones.
+// sigmoid(f) and 1 - sigmoid(f), each to the last bits: the smaller one is not the difference of two near ones.  1 + e lies in [1, 2], where the
+// approximate reciprocal is within one unit of the last place and a division of its own is not needed.
 __device__ __forceinline__ void gate(float f, float& a, float& rest) {
-  const float e = expf(-fabsf(f)), large = 1.f / (1.f + e), small = e * large;
+  const float e = expf(-fabsf(f));
+  float large;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(large) : "f"(1.f + e));
+  const float small = e * large;
   a = f < 0.f ? small : large;
   rest = f < 0.f ? large : small;
 }
@@ -92,6 +113,369 @@ __global__ void __launch_bounds__(kThreads) scan_columns_backward_kernel(const S
   if (s.dh0) s.dh0[col] = carry;
 }
 
+// ---- stretches ------------------------------------------------------------------------------------------------------------------------
+// A block has C = 16 or 32 columns.  A thread has V of them (128-bit accesses where everything is aligned, V = 4) and S timesteps, a warp several
+// units of C / V lanes one after the other in time; then come the warps of a block and the blocks of a cluster (backward: against time).
+constexpr int kMaxWarps = 8, kMaxCluster = 8;
+struct Exchange {
+  float2 of_warp[kMaxWarps][32];                // A and B
+  float2 of_block[2][kMaxCluster][32];          // of the cluster's blocks, turn by turn
+  uint64_t arrived[2];                          // barriers that count the bytes of those
+};
+template <int V>
+struct Vec;
+template <>
+struct Vec<1> {
+  static __device__ __forceinline__ void load(float (&v)[1], const float* p) { v[0] = __ldcs(p); }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
+};
+template <>
+struct Vec<4> {
+  static __device__ __forceinline__ void load(float (&v)[4], const float* p) {
+    const float4 q = __ldcs(reinterpret_cast<const float4*>(p));
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+};
+// What the blocks of a cluster tell one another goes by asynchronous stores, which a barrier in the receiver's shared memory counts: a barrier of
+// the whole cluster would wait for the results of the stretch before to be in memory, too (65536 timesteps of 512 columns: 112 us with it).
+// Two turns: a block may be one ahead of another that still reads, not two, since it needs what that one sends after reading.
+__device__ __forceinline__ void begin_exchange(Exchange& x) {
+  if (threadIdx.x == 0) {
+    tc::mbar_init(tc::smem_u32(&x.arrived[0]), 1);
+    tc::mbar_init(tc::smem_u32(&x.arrived[1]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  cg::this_cluster().sync();
+}
+__device__ __forceinline__ void send(const float2* place, const uint64_t* barrier, uint32_t to, float a, float b) {
+  asm volatile(
+      "{\n\t.reg .b32 p, q;\n\t.reg .b64 v;\n\t"
+      "mapa.shared::cluster.u32 p, %0, %2;\n\t"
+      "mapa.shared::cluster.u32 q, %1, %2;\n\t"
+      "mov.b64 v, {%3, %4};\n\t"
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [p], v, [q];\n\t}" ::"r"(tc::smem_u32(place)),
+      "r"(tc::smem_u32(barrier)), "r"(to), "f"(a), "f"(b)
+      : "memory");
+}
+// Until this turn's bytes are there, which other blocks of the cluster have written; bounded.
+__device__ __forceinline__ void receive(const uint64_t* barrier, uint32_t parity, int* status) {
+  for (uint32_t i = 0; i < tc::kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(barrier)), "r"(parity)
+        : "memory");
+    if (ok) return;
+  }
+  tc::record_status(status, 82);
+}
+// From the A and B of this thread's timesteps to the state that they start from.  `state`: of column `lane` before the cluster's stretch, afterwards
+// before its next one.
+template <int C, int V, bool CLUSTER>
+__device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const float (&b)[V], int blocks, int rank, int turn, int* status, float& state,
+                                         float (&from)[V]) {
+  constexpr int kLanes = C / V, kUnits = 32 / kLanes;  // lanes of a unit, units of a warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, unit = lane / kLanes;
+  float pa[V], pb[V], ea[V], eb[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {  // over the warp's units: inclusive, then of those before
+    pa[j] = a[j];
+    pb[j] = b[j];
+#pragma unroll
+    for (int o = kLanes; o < 32; o *= 2) {
+      const float qa = __shfl_up_sync(0xffffffffu, pa[j], o), qb = __shfl_up_sync(0xffffffffu, pb[j], o);
+      if (lane >= o) {
+        pb[j] = pa[j] * qb + pb[j];
+        pa[j] = pa[j] * qa;
+      }
+    }
+    ea[j] = 1.f;
+    eb[j] = 0.f;
+    if (kUnits > 1) {
+      const float qa = __shfl_up_sync(0xffffffffu, pa[j], kLanes), qb = __shfl_up_sync(0xffffffffu, pb[j], kLanes);
+      if (unit > 0) {
+        ea[j] = qa;
+        eb[j] = qb;
+      }
+    }
+  }
+  if (unit == kUnits - 1) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x.of_warp[warp][lane % kLanes * V + j] = make_float2(pa[j], pb[j]);
+  }
+  __syncthreads();
+  // from here on the lane is the column (lanes beyond C: nobody asks for theirs)
+  float wa = 1.f, wb = 0.f, ba = 1.f, bb = 0.f;  // of the warps before this one, of all
+  for (int w = 0; w < warps; ++w) {
+    if (w == warp) {
+      wa = ba;
+      wb = bb;
+    }
+    const float2 q = x.of_warp[w][lane];
+    bb = q.x * bb + q.y;
+    ba = q.x * ba;
+  }
+  float before = state;
+  if (CLUSTER) {
+    const int slot = turn & 1;
+    if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&x.arrived[slot]), blocks * 32 * (uint32_t)sizeof(float2));
+    for (int to = warp; to < blocks; to += warps) send(&x.of_block[slot][rank][lane], &x.arrived[slot], to, ba, bb);
+    receive(&x.arrived[slot], turn >> 1 & 1, status);
+    for (int r = 0; r < blocks; ++r) {
+      if (r == rank) before = state;
+      const float2 q = x.of_block[slot][r][lane];
+      state = q.x * state + q.y;
+    }
+  } else {
+    state = ba * state + bb;
+    __syncthreads();  // of_warp is written again
+  }
+  before = wa * before + wb;
+#pragma unroll
+  for (int j = 0; j < V; ++j) from[j] = ea[j] * __shfl_sync(0xffffffffu, before, lane % kLanes * V + j) + eb[j];
+}
+
+template <int C, int V, int S, bool CLUSTER>
+__global__ void __launch_bounds__(kMaxWarps * 32, CLUSTER ? 2 : 4) scan_stretches_kernel(const ScanArgs s, int blocks) {
+  RT_PDL_ENTRY();
+  __shared__ Exchange x;
+  constexpr int kLanes = C / V;
+  const int rank = CLUSTER ? blockIdx.x % blocks : 0, lane = threadIdx.x & 31;
+  const int64_t columns = s.batch * s.hidden, col0 = (int64_t)(CLUSTER ? blockIdx.x / blocks : blockIdx.x) * C, col = col0 + lane % kLanes * V;
+  const bool in = col < columns;
+  const int64_t step = s.batch * s.ld, at = in ? col / s.hidden * s.ld + col % s.hidden : 0;
+  const int units = blockDim.x / kLanes;
+  const int64_t all = (int64_t)blocks * units * S;  // timesteps of the cluster
+  int64_t t = ((int64_t)rank * units + threadIdx.x / kLanes) * S;
+  const float *f = s.f + at + t * step, *v = s.v + at + t * step;
+  float* h = s.h + col + t * columns;
+  float fs[S][V], vs[S][V];
+  int left;
+  auto load = [&] {
+    left = in ? (int)max((int64_t)0, min((int64_t)S, s.steps - t)) : 0;
+    const float *pf = f, *pv = v;
+    if (left == S) {
+#pragma unroll
+      for (int k = 0; k < S; ++k, pf += step, pv += step) {
+        Vec<V>::load(fs[k], pf);
+        Vec<V>::load(vs[k], pv);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < S; ++k, pf += step, pv += step) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        fs[k][j] = INFINITY;  // which leaves the state as it is
+        vs[k][j] = 0.f;
+      }
+      if (k < left) {
+        Vec<V>::load(fs[k], pf);
+        Vec<V>::load(vs[k], pv);
+      }
+    }
+  };
+  float state = s.h0 && lane < C && col0 + lane < columns ? __ldg(s.h0 + col0 + lane) : 0.f;
+  if (CLUSTER) {  // elsewhere the other blocks of the SM keep the memory busy
+    load();
+    begin_exchange(x);
+  }
+  int turn = 0;
+  for (int64_t t0 = 0; t0 < s.steps; t0 += all, ++turn) {
+    if (!CLUSTER) load();
+    float a[S][V], b[S][V];  // from the thread's first timestep on
+#pragma unroll
+    for (int k = 0; k < S; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float rest;
+        gate(fs[k][j], a[k][j], rest);
+        b[k][j] = rest * vs[k][j];
+        if (k > 0) {
+          b[k][j] += a[k][j] * b[k - 1][j];
+          a[k][j] *= a[k - 1][j];
+        }
+      }
+    const int mine = left;
+    t += all;
+    f += all * step;
+    v += all * step;
+    if (CLUSTER && t0 + all < s.steps) load();
+    float from[V];
+    start_of<C, V, CLUSTER>(x, a[S - 1], b[S - 1], blocks, rank, turn, s.status, state, from);
+    float* ph = h;
+#pragma unroll
+    for (int k = 0; k < S; ++k, ph += columns) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) b[k][j] += a[k][j] * from[j];
+      if (k < mine) Vec<V>::store(ph, b[k]);
+    }
+    h += all * columns;
+  }
+  if (CLUSTER) cg::this_cluster().sync();  // nobody leaves while another may still send to it
+}
+
+// The same against time, for e_t = a_t d_t = a_t e_{t+1} + a_t dh_t, from which d_t = dh_t + e_{t+1}.
+template <int C, int V, int S, bool CLUSTER>
+__global__ void __launch_bounds__(kMaxWarps * 32, CLUSTER ? 2 : 4) scan_stretches_backward_kernel(const ScanArgs s, int blocks) {
+  RT_PDL_ENTRY();
+  __shared__ Exchange x;
+  constexpr int kLanes = C / V;
+  const int rank = CLUSTER ? blockIdx.x % blocks : 0, lane = threadIdx.x & 31;
+  const int64_t columns = s.batch * s.hidden, col0 = (int64_t)(CLUSTER ? blockIdx.x / blocks : blockIdx.x) * C, col = col0 + lane % kLanes * V;
+  const bool in = col < columns;
+  const int64_t step = s.batch * s.ld, step_out = s.batch * s.ldd;
+  const int64_t at = in ? col / s.hidden * s.ld + col % s.hidden : 0, at_out = in ? col / s.hidden * s.ldd + col % s.hidden : 0;
+  const int units = blockDim.x / kLanes;
+  const int64_t all = (int64_t)blocks * units * S;
+  int64_t t = s.steps - 1 - ((int64_t)rank * units + threadIdx.x / kLanes) * S;  // the thread's last timestep, with which it begins
+  const float *f = s.f + at + t * step, *v = s.v + at + t * step, *h = s.states + col + (t - 1) * columns, *g = s.dh + col + t * columns;
+  float *df = s.df + at_out + t * step_out, *dv = s.dv + at_out + t * step_out;
+  float fs[S][V], vs[S][V], hs[S][V], gs[S][V];
+  int left;
+  auto load = [&] {
+    left = in ? (int)max((int64_t)0, min((int64_t)S, t + 1)) : 0;
+    const float *pf = f, *pv = v, *ph = h, *pg = g;
+    if (left == S && t >= S) {
+#pragma unroll
+      for (int k = 0; k < S; ++k, pf -= step, pv -= step, ph -= columns, pg -= columns) {
+        Vec<V>::load(fs[k], pf);
+        Vec<V>::load(vs[k], pv);
+        Vec<V>::load(gs[k], pg);
+        Vec<V>::load(hs[k], ph);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < S; ++k, pf -= step, pv -= step, ph -= columns, pg -= columns) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        fs[k][j] = INFINITY;
+        vs[k][j] = hs[k][j] = gs[k][j] = 0.f;
+      }
+      if (k < left) {
+        Vec<V>::load(fs[k], pf);
+        Vec<V>::load(vs[k], pv);
+        Vec<V>::load(gs[k], pg);
+        if (t > k) Vec<V>::load(hs[k], ph);
+        else if (s.h0) Vec<V>::load(hs[k], s.h0 + col);
+      }
+    }
+  };
+  float state = 0.f;
+  if (CLUSTER) {  // elsewhere the other blocks of the SM keep the memory busy
+    load();
+    begin_exchange(x);
+  }
+  int turn = 0;
+  for (int64_t t0 = 0; t0 < s.steps; t0 += all, ++turn) {
+    if (!CLUSTER) load();
+    float da[S][V], db[S][V], slope[S][V], rest[S][V], ea[V], eb[V];  // d = da * (e behind the thread's timesteps) + db
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ea[j] = 1.f;
+      eb[j] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < S; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float a;
+        gate(fs[k][j], a, rest[k][j]);
+        slope[k][j] = (hs[k][j] - vs[k][j]) * a * rest[k][j];
+        da[k][j] = ea[j];
+        db[k][j] = gs[k][j] + eb[j];
+        ea[j] = a * da[k][j];
+        eb[j] = a * db[k][j];
+      }
+    const int mine = left;
+    t -= all;
+    f -= all * step;
+    v -= all * step;
+    h -= all * columns;
+    g -= all * columns;
+    if (CLUSTER && t0 + all < s.steps) load();
+    float from[V];
+    start_of<C, V, CLUSTER>(x, ea, eb, blocks, rank, turn, s.status, state, from);
+    float *pf = df, *pv = dv;
+#pragma unroll
+    for (int k = 0; k < S; ++k, pf -= step_out, pv -= step_out) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = da[k][j] * from[j] + db[k][j];
+        slope[k][j] *= d;
+        rest[k][j] *= d;
+      }
+      if (k < mine) {
+        Vec<V>::store(pf, slope[k]);
+        Vec<V>::store(pv, rest[k]);
+      }
+    }
+    df -= all * step_out;
+    dv -= all * step_out;
+  }
+  if (CLUSTER) cg::this_cluster().sync();
+  if (s.dh0 && rank == 0 && threadIdx.x < C && col0 + lane < columns) s.dh0[col0 + lane] = state;
+}
+
+// How a sequence is cut: columns and warps of a block, blocks of a cluster.  Clusters while the columns alone do not occupy the SMs; strips of 16
+// columns (64 bytes of a row) while those of 32 leave half of the SMs without a second block.
+struct Cut {
+  int columns, warps, blocks;
+  int64_t strips;
+};
+Cut cut(const rt_ctx* ctx, int64_t steps, int64_t columns, int thread_values) {
+  for (int width = 32;; width = 16) {
+    const int warp_steps = thread_values * 32 / width;
+    const int64_t strips = (columns + width - 1) / width, stretches = (steps + warp_steps - 1) / warp_steps;
+    const int warps = (int)(stretches < kMaxWarps ? stretches : kMaxWarps);
+    int blocks = 1;
+    while (blocks < kMaxCluster && strips * blocks < 2 * ctx->sm_count && blocks * warps < stretches) blocks *= 2;
+    if (width == 16 || blocks < kMaxCluster || strips * blocks > ctx->sm_count) return {width, warps, blocks, strips};
+  }
+}
+template <class Kernel>
+rt_status launch_stretches(rt_ctx* ctx, Kernel kern, const ScanArgs& s, const Cut& c) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = (unsigned)(c.strips * c.blocks);
+  cfg.blockDim = (unsigned)c.warps * 32;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)c.blocks;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = c.blocks > 1 ? 2 : 1;
+  RT_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, s, c.blocks));
+  RT_LAUNCHED(ctx);
+  return RT_OK;
+}
+template <int V, int S>
+rt_status launch_forward(rt_ctx* ctx, const ScanArgs& s) {
+  const Cut c = cut(ctx, s.steps, s.batch * s.hidden, V * S);
+  if (c.columns == 16) return launch_stretches(ctx, scan_stretches_kernel<16, V, S, true>, s, c);
+  return c.blocks > 1 ? launch_stretches(ctx, scan_stretches_kernel<32, V, S, true>, s, c) : launch_stretches(ctx, scan_stretches_kernel<32, V, S, false>, s, c);
+}
+template <int V, int S>
+rt_status launch_backward(rt_ctx* ctx, const ScanArgs& s) {
+  const Cut c = cut(ctx, s.steps, s.batch * s.hidden, V * S);
+  if (c.columns == 16) return launch_stretches(ctx, scan_stretches_backward_kernel<16, V, S, true>, s, c);
+  return c.blocks > 1 ? launch_stretches(ctx, scan_stretches_backward_kernel<32, V, S, true>, s, c)
+                      : launch_stretches(ctx, scan_stretches_backward_kernel<32, V, S, false>, s, c);
+}
+// Whether four columns of every matrix can be had at once.
+bool aligned(const ScanArgs& s) {
+  bool ok = s.hidden % 4 == 0 && s.ld % 4 == 0 && s.ldd % 4 == 0;
+  for (const float* p : {s.f, s.v, s.h0, (const float*)s.h, s.states, s.dh, (const float*)s.df, (const float*)s.dv}) ok = ok && rt_aligned16(p);
+  return ok;
+}
+
 rt_status check_sizes(rt_ctx* ctx, const char* who, int64_t steps, int64_t batch, int64_t hidden, int64_t ld) {
   if (steps < 0 || batch < 0 || hidden < 0) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "%s: negative size", who);
   if (ld < hidden) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "%s: rows of %lld values, %lld apart", who, (long long)hidden, (long long)ld);
@@ -124,6 +508,8 @@ rt_status rt_gated_scan(rt_ctx* ctx, const float* f, const float* v, int64_t ld,
   s.batch = batch;
   s.hidden = hidden;
   s.h = h;
+  s.status = ctx->device_status;
+  if (steps > kAhead) return aligned(s) ? launch_forward<4, 4>(ctx, s) : launch_forward<1, 16>(ctx, s);
   rt_launch(ctx, scan_columns_kernel, (unsigned)((batch * hidden + kThreads - 1) / kThreads), kThreads, 0, s);
   RT_LAUNCHED(ctx);
   return RT_OK;
@@ -158,6 +544,8 @@ rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, in
   s.dv = dv;
   s.ldd = ldd;
   s.dh0 = dh0;
+  s.status = ctx->device_status;
+  if (steps > kAhead) return aligned(s) ? launch_backward<4, 2>(ctx, s) : launch_backward<1, 8>(ctx, s);
   rt_launch(ctx, scan_columns_backward_kernel, (unsigned)((batch * hidden + kThreads - 1) / kThreads), kThreads, 0, s);
   RT_LAUNCHED(ctx);
   return RT_OK;

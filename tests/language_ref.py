@@ -32,9 +32,10 @@ def sigmoid(f):
     return np.where(f >= 0, 1, e) / (1 + e), np.where(f >= 0, e, 1) / (1 + e)
 
 
-# A gate: expf within 2 U of itself, of which 1 + e keeps at most half (1 U) and adds 1, a division 1; the smaller one once more e (2) and a
-# product (1): 6 U.  A timestep multiplies with it and adds: 8 U for each timestep that a term has passed, however the timesteps are grouped.
-GATE, STEP = 6, 8
+# A gate: expf within 2 U of itself, of which 1 + e keeps at most half (1 U) and adds 1, an approximate reciprocal 2 (one unit of the last place);
+# the smaller one once more e (2) and a product (1): 7 U.  A timestep multiplies with it and adds: 9 U for each timestep that a term has
+# passed, however the timesteps are grouped.
+GATE, STEP = 7, 9
 
 
 def scan(f, v, h0):
