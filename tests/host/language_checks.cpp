@@ -56,7 +56,8 @@ int main() {
   EXPECT(rt_gated_scan_backward(&ctx, x, x, 2, nullptr, x, x, 0, 1, 2, x, x, 2, nullptr) == RT_OK);
   // Muon
   float *p[2] = {x, x + 32}, *m[2] = {x + 16, x + 48}, *none[2] = {x, nullptr};
-  const float* g[2] = {x, x};
+  float y[32] = {};
+  const float* g[2] = {y, y};
   const int64_t rows[2] = {4, 2}, cols[2] = {4, 3}, negative[2] = {4, -2}, large[2] = {4, 1 << 24};
   EXPECT(REFUSED(rt_muon_step_multi(&ctx, -1, p, g, m, rows, cols, 0.1f, 0.9f, 0, 0.f, 5, 1.f), "matrices"));
   EXPECT(REFUSED(rt_muon_step_multi(&ctx, 2, p, g, m, rows, cols, 0.1f, 0.9f, 0, 0.f, -1, 1.f), "steps"));
@@ -69,8 +70,15 @@ int main() {
   float *twice[2] = {x, x + 12};
   EXPECT(REFUSED(rt_muon_step_multi(&ctx, 2, twice, g, m, rows, cols, 0.1f, 0.9f, 0, 0.f, 5, 1.f), "overlap"));
   EXPECT(REFUSED(rt_muon_step_multi(&ctx, 2, p, g, p, rows, cols, 0.1f, 0.9f, 0, 0.f, 5, 1.f), "overlap"));
+  const float* of_m[2] = {x, x + 40};  // the second within a parameter
+  float* q[2] = {x + 20, x + 40};
+  EXPECT(REFUSED(rt_muon_step_multi(&ctx, 2, q, of_m, m, rows, cols, 0.1f, 0.9f, 0, 0.f, 5, 1.f), "overlap"));
+  const int64_t tall[2] = {4, 65537}, wide[2] = {4, 65537};
+  EXPECT(REFUSED(rt_muon_step_multi(&ctx, 2, p, g, m, tall, wide, 0.1f, 0.9f, 0, 0.f, 5, 1.f), "out of range"));
   EXPECT(rt_muon_step_multi(&ctx, 0, nullptr, nullptr, nullptr, nullptr, nullptr, 0.1f, 0.9f, 0, 0.f, 5, 1.f) == RT_OK);
   EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, g, rows, cols, 5, twice), "overlap"));
+  float* onto[2] = {y + 8, x};  // a result within the other's matrix
+  EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, g, rows, cols, 5, onto), "overlap"));
   EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, g, rows, cols, 5, none), "outs"));
   EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 1, g, nullptr, cols, 5, p), "rows"));
   EXPECT(ctx.launches == 0);

@@ -260,10 +260,10 @@ def test_orthogonalize(capi, steps):
         if steps == 5 and min(x.shape) < 100 < max(x.shape):  # far from square: no tiny singular values
             s = np.linalg.svd(o, compute_uv=False)
             assert 0.6 < s.min() and s.max() < 1.25
-    # in place, each by itself: what is in a list beside a matrix changes nothing
-    for x, dx, o in zip(xs, d, got):
+    # in place, each by itself (how the reductions are shared among blocks, and so the last bits, goes by the whole list)
+    for x, dx in zip(xs, d):
         capi.call("orthogonalize_list", 1, pointers([dx]), capi.i64([x.shape[0]]), capi.i64([x.shape[1]]), steps, pointers([dx]))
-        assert np.array_equal(dx.numpy().ravel(), o[: x.size])
+        as_near_as_fp32(dx.numpy(), ref.orthogonalize(x, steps), ref.orthogonalize(x, steps, np.float32))
 
 
 @pytest.mark.parametrize("value", [0.0, 1e-30, 1e30, np.nan, np.inf])
