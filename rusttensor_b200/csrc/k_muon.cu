@@ -8,11 +8,15 @@
 //
 // A step is three products, each of which has to wait for the one before: G = X X^T and b G + c G^2, both symmetric, of which the lower half is
 // computed and written twice, and a X + (b G + c G^2) X.  Errors of early steps grow (small singular values by 3.4 a step), so the products
-// keep fp32's precision: an operand is held as two fp16 parts, hi = fp16(2^12 x) and lo = fp16(2^11 (2^12 x - hi)), 22 bits, and a product is
-// three tcgen05.mma of kind::f16, hi hi to one accumulator, hi lo and lo hi to another.  No element of X, G or the polynomial is beyond 3 (their
-// singular values are at most 1.21, 1.46 and 2.81), so the scale is fixed and nothing is looked at beforehand.  A product's epilogue adds what
+// keep fp32's precision: an operand is held as two fp16 parts, hi = fp16(2^12 x) and lo = fp16(2^12 x - hi), 22 bits, and a product is three
+// tcgen05.mma of kind::f16: hi lo, lo hi and hi hi.  No element of X, G or the polynomial is beyond 3 (their singular values are at most 1.21,
+// 1.46 and 2.81), so the scale is fixed and nothing is looked at beforehand; below 2^-15, where lo has fewer than 11 bits left, an element is
+// off by 2^-37 at most.  A product's epilogue adds what
 // the formula adds and writes the parts that the next product reads, as they lie: X [m][n] is an operand with n as the reduction, and with
-// m, by tensor maps and MMA descriptors of either kind.  All matrices of a call go through every product together, as tiles of one launch.
+// m, by tensor maps and MMA descriptors of either kind.  All matrices of a call go through every product together, and all products are one
+// cooperative launch, whose blocks wait for one another between two products (15 launches for five steps were 4 us each besides the work).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -25,7 +29,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr double kEpsilon = 1e-7;
-constexpr int kNormBlocks = 128;
+constexpr int kNormBlocks = 256;
 
 struct Update {
   const float* x;  // what is orthogonalised; with a gradient: made of it and the momentum
@@ -38,31 +42,90 @@ __device__ __forceinline__ float update_at(const Update& u, int64_t i) {
   if (!u.g) return __ldg(u.x + i);
   return u.nesterov ? u.scale * __ldg(u.g + i) + u.mu * u.m[i] : u.m[i];
 }
-// The new momentum, and the sum of the squares of the update, block by block in 64 bits: squares of large fp32 values have no room in 32.
-__global__ void __launch_bounds__(kThreads) squares_kernel(const Update u, int64_t n, double* __restrict__ sums) {
+// The new momentum, and the sum of the squares of the update, block by block in 64 bits: squares of large fp32 values have no room in 32.  A
+// matrix has kNormBlocks blocks.  Bound by memory: 4096 x 4096 takes 17 us (236 with one value at a time in 128 blocks).
+constexpr int kGroup = 12;  // matrices of a launch
+struct Squares {
+  Update u[kGroup];
+  int64_t n[kGroup];
+  double* sums;  // [matrix][block]
+};
+template <bool VEC>
+__device__ __forceinline__ double sum_of_squares(const Update& u, int64_t n) {
+  constexpr int kAhead = 4, V = VEC ? 4 : 1;
+  double sum = 0.0;
+  const int64_t step = (int64_t)kNormBlocks * kThreads * V;
+  for (int64_t i0 = ((int64_t)(blockIdx.x % kNormBlocks) * kThreads + threadIdx.x) * V; i0 < n; i0 += kAhead * step) {
+    float g[kAhead][V], m[kAhead][V];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * step;
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[k][j] = m[k][j] = 0.f;
+      if (i >= n) continue;
+      const float *from = (u.g ? u.g : u.x) + i, *old = u.m + i;
+      if (VEC) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(from));
+        g[k][0] = q.x; g[k][V / 4] = q.y; g[k][V / 2] = q.z; g[k][V - 1] = q.w;
+        if (u.g) {
+          const float4 r = *reinterpret_cast<const float4*>(old);
+          m[k][0] = r.x; m[k][V / 4] = r.y; m[k][V / 2] = r.z; m[k][V - 1] = r.w;
+        }
+      } else {
+        g[k][0] = __ldg(from);
+        if (u.g) m[k][0] = *old;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * step;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        double v = g[k][j];
+        if (u.g) {
+          m[k][j] = u.mu * m[k][j] + u.scale * g[k][j];
+          v = u.nesterov ? u.scale * g[k][j] + u.mu * m[k][j] : m[k][j];
+        }
+        sum += v * v;
+      }
+      if (u.g && i < n) {
+        if (VEC) *reinterpret_cast<float4*>(u.m + i) = make_float4(m[k][0], m[k][V / 4], m[k][V / 2], m[k][V - 1]);
+        else u.m[i] = m[k][0];
+      }
+    }
+  }
+  return sum;
+}
+__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Squares p) {
   RT_PDL_ENTRY();
   __shared__ double of_warp[kThreads / 32];
-  double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-    if (u.g) u.m[i] = u.mu * u.m[i] + u.scale * __ldg(u.g + i);
-    const double v = update_at(u, i);
-    sum += v * v;
-  }
+  const int q = blockIdx.x / kNormBlocks;
+  const Update u = p.u[q];
+  const int64_t n = p.n[q];
+  const bool vec = n % 4 == 0 && (((uintptr_t)u.x | (uintptr_t)u.g | (uintptr_t)u.m) & 15) == 0;
+  double sum = vec ? sum_of_squares<true>(u, n) : sum_of_squares<false>(u, n);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kThreads / 32; ++w) sum += of_warp[w];
-    sums[blockIdx.x] = sum;
+    p.sums[blockIdx.x] = sum;
   }
+}
+// 1 / (norm + epsilon), in every thread of a warp.
+__device__ __forceinline__ float one_over_norm(const double* __restrict__ sums) {
+  double sum = 0.0;
+#pragma unroll
+  for (int b = 0; b < kNormBlocks; b += 32) sum += __ldg(sums + b + (threadIdx.x & 31));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return (float)(1.0 / (sqrt(sum) + kEpsilon));
 }
 // X: the update divided by its norm, its shorter side first.
 __global__ void __launch_bounds__(kThreads) normalise_kernel(const Update u, int64_t rows, int64_t cols, const double* __restrict__ sums, float* __restrict__ x) {
   RT_PDL_ENTRY();
-  double sum = 0.0;
-  for (int b = 0; b < kNormBlocks; ++b) sum += __ldg(sums + b);
-  const float by = (float)(1.0 / (sqrt(sum) + kEpsilon));
+  const float by = one_over_norm(sums);
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * kThreads) {
     const int64_t r = i / cols, c = i - r * cols;
     x[rows > cols ? c * rows + r : i] = update_at(u, i) * by;
@@ -93,86 +156,241 @@ struct Matrix {
   float keep, step;
 };
 
+rt_status launch_squares(rt_ctx* ctx, const Matrix* list, int count, double* sums) {
+  Squares p{};
+  for (int q = 0; q < count; ++q) {
+    p.u[q] = list[q].u;
+    p.n[q] = list[q].rows * list[q].cols;
+  }
+  p.sums = sums;
+  rt_launch(ctx, squares_kernel, kNormBlocks * count, kThreads, 0, p);
+  RT_LAUNCHED(ctx);
+  return RT_OK;
+}
+
 // ---- the products on the tensor cores -----------------------------------------------------------------------------------------------
 using namespace tc;
+namespace cg = cooperative_groups;
 using parts::kBox;
 
-constexpr int kGroup = 16;                 // matrices of a launch
-constexpr float kScale = 4096.f, kLow = 2048.f;
+constexpr float kScale = 4096.f;
 constexpr int kTileM = 128, kBlockK = 64;  // rows of a tile; elements of the reduction that a stage holds
-constexpr int kProductThreads = 320, kEpilogueWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
-constexpr uint32_t kCross = 256;           // tensor-memory column of the cross terms
-enum { kGram, kSquare, kApply };
+constexpr uint32_t kSecond = 256;          // tensor-memory column of the second accumulator
+enum { kGram, kSquare, kApply, kResult };  // kResult: the last kApply, whose result goes to `out`
 
 struct Item {
   int m, n;              // m <= n
   int ldx, ldm;          // halves between rows of X, of G and the polynomial
   uint16_t *x[2], *g, *s;
-  int first, splits;     // of this product: first work item of the matrix, CTAs that share a tile's reduction
-  int first_part;        // tile partial sums of matrices before, in tiles
-  int first_ticket;
+  int first[3], splits[3];  // by product: first work item of the matrix, CTAs that share a tile's reduction
+  int first_part[3];        // partial sums of the matrices before, in tiles
+  int first_ticket[3];
   // the result
   float* out;
-  int tall, update;      // X is transposed against out
+  int tall, update, vec; // X is transposed against out; 128-bit accesses to out
   float keep, step;
 };
 struct Product {
-  CUtensorMap x[2][kGroup], g[kGroup], s[kGroup];
+  // X, G and the polynomial, both planes in a box: 128 rows high as left operands, as right ones as many as a CTA brings in, X 64 as the right operand
+  // whose rows are the reduction.
+  CUtensorMap x_left[2][kGroup], x_right[2][kGroup], x_apply[2][kGroup], g_left[kGroup], g_right[kGroup], s_left[kGroup];
   Item item[kGroup];
-  int count, items;
-  int from;              // which of the two X is read
-  int last;              // the result goes to `out`
-  int chunk;             // K-blocks that the accumulator of hi * hi sums before it is emptied: it adds with truncation
-  float* sums;           // partial sums of tiles, [128 columns or 256][128 rows] each
-  unsigned* tickets;     // zero between launches
+  int count, steps;
+  int items[3];
+  float* sums;           // partial sums of tiles, [columns][128 rows] each
+  unsigned* tickets;     // zero
+  unsigned* arrived;     // zero; blocks that have done their part, of all products
   int* status;
 };
-template <int W>
-struct Smem {
-  static constexpr uint32_t stage = (2 * kTileM + 2 * W) / 64 * kBox, stages = W == 256 ? 2 : 3;
-  static constexpr uint32_t bars = stages * stage, bytes = bars + (2 * stages + 3) * 8 + 16 + 1024;
+// Results are finished by slabs of 64 columns.
+constexpr int kSlab = 64;
+// A tile of W columns has 128 rows and belongs to a CTA, or (PAIR) 256 rows and belongs to two CTAs of a cluster: each has 128 of the rows and
+// brings in half of the right operand, which the MMAs of a pair read from both.
+template <int W, bool PAIR>
+struct Layout {
+  static constexpr int rows = PAIR ? 2 * kTileM : kTileM;
+  static constexpr int right = PAIR ? W / 2 : W;   // columns of the right operand that a CTA brings in
+  static constexpr int warps = 16;                 // that finish results; then one for TMA, one for the MMAs
+  static constexpr int tma = warps, mma = warps + 1, threads = (warps + 2) * 32;
+  static constexpr int cols = W * 4 / warps;       // of a warp
+  static constexpr uint32_t stage = (2 * kTileM + 2 * right) / 64 * kBox, stages = right == 128 ? 3 : 4;
+  static constexpr uint32_t slab = stages * stage;
+  static constexpr uint32_t bars = slab + kTileM * kSlab * 4, bytes = bars + (2 * stages + 5) * 8 + 16;
   static_assert(bytes <= 232448, "shared memory");
+  static_assert(W == rows || W == rows / 2, "tiles of the lower half");
 };
 struct Tile {
   int q, row, col, k0, k1, split, index;  // K-blocks k0 .. k1; index: among the matrix's tiles
 };
-template <int PHASE, int W>
-__device__ __forceinline__ Tile tile_of(const Product& p, int i) {
+// K-blocks that an accumulator sums before it is emptied into registers, because it adds with truncation.  After two a long reduction is nearer to the
+// exact result than one in fp32 (five steps of 4096 x 4096: 1.6e-6 and 4.9e-6 off); a short one needs the half of that (784 x 128: 1.7e-6, 1.6e-6 in
+// fp32), where it costs little.
+template <int W>
+__device__ __forceinline__ int chunk_of(int depth) { return W == 64 && depth < 1024 ? 1 : 2; }
+template <int W, bool PAIR>
+__device__ __forceinline__ Tile tile_of(const Product& p, int phase, int i) {
+  constexpr int rows = Layout<W, PAIR>::rows;
   int q = 0;
-  while (q + 1 < p.count && i >= p.item[q + 1].first) ++q;
+  while (q + 1 < p.count && i >= p.item[q + 1].first[phase]) ++q;
   const Item& a = p.item[q];
   Tile t;
   t.q = q;
-  const int local = i - a.first;
-  t.split = local % a.splits;
-  t.index = local / a.splits;
-  const int m_tiles = (a.m + kTileM - 1) / kTileM;
-  if (PHASE == kApply) {
-    t.row = t.index % m_tiles * kTileM;
+  const int local = i - a.first[phase], splits = a.splits[phase];
+  t.split = local % splits;
+  t.index = local / splits;
+  const int m_tiles = (a.m + rows - 1) / rows;
+  if (phase == kApply) {
+    t.row = t.index % m_tiles * rows;
     t.col = t.index / m_tiles * W;
-  } else if (W == kTileM) {  // the lower half, row by row: 1 + 2 + 3 + ... tiles
+  } else if (W == rows) {  // the lower half, row by row: 1 + 2 + 3 + ... tiles
     int r = (int)((sqrtf(8.f * t.index + 1.f) - 1.f) * 0.5f);
     while (r * (r + 1) / 2 > t.index) --r;
     while ((r + 1) * (r + 2) / 2 <= t.index) ++r;
-    t.row = r * kTileM;
+    t.row = r * rows;
     t.col = (t.index - r * (r + 1) / 2) * W;
-  } else {  // 1 + 1 + 2 + 2 + 3 + 3 + ...
+  } else {  // 2 + 4 + 6 + ...
     int r = (int)((sqrtf(4.f * t.index + 1.f) - 1.f) * 0.5f);
     while (r * (r + 1) > t.index) --r;
     while ((r + 1) * (r + 2) <= t.index) ++r;
-    const int in = t.index - r * (r + 1);
-    t.row = (2 * r + (in > r)) * kTileM;
-    t.col = (in > r ? in - r - 1 : in) * W;
+    t.row = r * rows;
+    t.col = (t.index - r * (r + 1)) * W;
   }
-  const int k_blocks = ((PHASE == kGram ? a.n : a.m) + kBlockK - 1) / kBlockK;
-  t.k0 = (int)((int64_t)k_blocks * t.split / a.splits);
-  t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / a.splits);
+  const int k_blocks = ((phase == kGram ? a.n : a.m) + kBlockK - 1) / kBlockK;
+  t.k0 = (int)((int64_t)k_blocks * t.split / splits);
+  t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / splits);
   return t;
 }
+// With PAIR the barrier is the one of the cluster's first CTA at the same place.
+template <bool PAIR>
 __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
-               "r"(x), "r"(y), "r"(z), "r"(bar)
-               : "memory");
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar & 0xFEFFFFFFu)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+// The MMAs before are done: for this CTA, or for both of a pair.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred pe;\n\t.reg .b16 m;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "mov.u16 m, 3;\n\t"
+        "@pe tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar)
+        : "memory");
+  else
+    umma_commit_elect(bar);
+}
+// At the barrier of the CTA that issues the MMAs.
+template <bool PAIR>
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .b32 r;\n\t"
+        "mapa.shared::cluster.u32 r, %0, 0;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar)
+        : "memory");
+  else
+    mbar_arrive(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void allocate(uint32_t slot) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, 512);
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void release(uint32_t tmem) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  else tmem_dealloc(tmem, 512);
+}
+// The MMAs of a K-block, in one statement: what they need is then moved to where they take it from all at once (one by one each took 71 cycles to
+// issue).  A slot of 16 of the reduction is 2 further in the left descriptor, `step_b` in the right one.  hi lo and lo hi come first: what is cut off of
+// them in an empty accumulator is as small as they are.  One elected lane of a converged warp issues.
+template <bool PAIR>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint32_t a_lo, uint32_t b, uint32_t b_lo, uint32_t step_b, uint32_t desc_hi, uint32_t idesc,
+                                          uint32_t more) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred pe, pm, pt;\n\t"
+        ".reg .b32 a1, a2, a3, b1, b2, b3, x1, x2, x3, y1, y2, y3;\n\t"
+        ".reg .b64 A0, A1, A2, A3, B0, B1, B2, B3, X0, X1, X2, X3, Y0, Y1, Y2, Y3;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "setp.ne.b32 pm, %8, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "add.u32 a1, %1, 2;\n\tadd.u32 a2, %1, 4;\n\tadd.u32 a3, %1, 6;\n\t"
+        "add.u32 x1, %2, 2;\n\tadd.u32 x2, %2, 4;\n\tadd.u32 x3, %2, 6;\n\t"
+        "add.u32 b1, %3, %5;\n\tadd.u32 b2, b1, %5;\n\tadd.u32 b3, b2, %5;\n\t"
+        "add.u32 y1, %4, %5;\n\tadd.u32 y2, y1, %5;\n\tadd.u32 y3, y2, %5;\n\t"
+        "mov.b64 A0, {%1, %6};\n\tmov.b64 A1, {a1, %6};\n\tmov.b64 A2, {a2, %6};\n\tmov.b64 A3, {a3, %6};\n\t"
+        "mov.b64 X0, {%2, %6};\n\tmov.b64 X1, {x1, %6};\n\tmov.b64 X2, {x2, %6};\n\tmov.b64 X3, {x3, %6};\n\t"
+        "mov.b64 B0, {%3, %6};\n\tmov.b64 B1, {b1, %6};\n\tmov.b64 B2, {b2, %6};\n\tmov.b64 B3, {b3, %6};\n\t"
+        "mov.b64 Y0, {%4, %6};\n\tmov.b64 Y1, {y1, %6};\n\tmov.b64 Y2, {y2, %6};\n\tmov.b64 Y3, {y3, %6};\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A0, Y0, %7, pm;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], X0, B0, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A1, Y1, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], X1, B1, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A2, Y2, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], X2, B2, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A3, Y3, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], X3, B3, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A0, B0, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A1, B1, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A2, B2, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], A3, B3, %7, pt;\n\t}" ::"r"(d),
+        "r"(a), "r"(a_lo), "r"(b), "r"(b_lo), "r"(step_b), "r"(desc_hi), "r"(idesc), "r"(more)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred pe, pm, pt;\n\t"
+        ".reg .b32 a1, a2, a3, b1, b2, b3, x1, x2, x3, y1, y2, y3;\n\t"
+        ".reg .b64 A0, A1, A2, A3, B0, B1, B2, B3, X0, X1, X2, X3, Y0, Y1, Y2, Y3;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "setp.ne.b32 pm, %8, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "add.u32 a1, %1, 2;\n\tadd.u32 a2, %1, 4;\n\tadd.u32 a3, %1, 6;\n\t"
+        "add.u32 x1, %2, 2;\n\tadd.u32 x2, %2, 4;\n\tadd.u32 x3, %2, 6;\n\t"
+        "add.u32 b1, %3, %5;\n\tadd.u32 b2, b1, %5;\n\tadd.u32 b3, b2, %5;\n\t"
+        "add.u32 y1, %4, %5;\n\tadd.u32 y2, y1, %5;\n\tadd.u32 y3, y2, %5;\n\t"
+        "mov.b64 A0, {%1, %6};\n\tmov.b64 A1, {a1, %6};\n\tmov.b64 A2, {a2, %6};\n\tmov.b64 A3, {a3, %6};\n\t"
+        "mov.b64 X0, {%2, %6};\n\tmov.b64 X1, {x1, %6};\n\tmov.b64 X2, {x2, %6};\n\tmov.b64 X3, {x3, %6};\n\t"
+        "mov.b64 B0, {%3, %6};\n\tmov.b64 B1, {b1, %6};\n\tmov.b64 B2, {b2, %6};\n\tmov.b64 B3, {b3, %6};\n\t"
+        "mov.b64 Y0, {%4, %6};\n\tmov.b64 Y1, {y1, %6};\n\tmov.b64 Y2, {y2, %6};\n\tmov.b64 Y3, {y3, %6};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A0, Y0, %7, pm;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], X0, B0, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A1, Y1, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], X1, B1, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A2, Y2, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], X2, B2, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A3, Y3, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], X3, B3, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A0, B0, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A1, B1, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A2, B2, %7, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], A3, B3, %7, pt;\n\t}" ::"r"(d),
+        "r"(a), "r"(a_lo), "r"(b), "r"(b_lo), "r"(step_b), "r"(desc_hi), "r"(idesc), "r"(more)
+        : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_one(uint32_t d, uint32_t a, uint32_t b, uint32_t desc_hi, uint32_t idesc, uint32_t more) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred pa, pe;\n\t.reg .b64 da, db;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "setp.ne.b32 pa, %5, 0;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "@pe tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, pa;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(desc_hi), "r"(idesc), "r"(more)
+        : "memory");
+  else
+    parts::mma(d, a, desc_hi, b, desc_hi, idesc, more);
 }
 // Two neighbouring values as parts.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -180,268 +398,393 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   b *= kScale;
   const __half2 h = __floats2half2_rn(a, b);
   const float2 back = __half22float2(h);
-  const __half2 l = __floats2half2_rn((a - back.x) * kLow, (b - back.y) * kLow);
+  const __half2 l = __floats2half2_rn(a - back.x, b - back.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 __device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi)), l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-  return make_float2((h.x + l.x * (1.f / kLow)) * (1.f / kScale), (h.y + l.y * (1.f / kLow)) * (1.f / kScale));
+  return make_float2((h.x + l.x) * (1.f / kScale), (h.y + l.y) * (1.f / kScale));
 }
-// What of eight values of a row is added to the product: `by` times what the parts at p (hi; lo a plane behind) hold.
-__device__ __forceinline__ void add_parts(float (&v)[8], const uint16_t* p, int64_t plane, float by) {
-  const uint4 h = *reinterpret_cast<const uint4*>(p), l = *reinterpret_cast<const uint4*>(p + plane);
-  const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 f = join2(hs[k], ls[k]);
-    v[2 * k] += by * f.x;
-    v[2 * k + 1] += by * f.y;
+// A CTA's 128 x 64 results in shared memory, four columns a piece; where a row has its pieces keeps apart what is accessed together: the same
+// piece of eight rows in a row, and of every fourth one.
+__device__ __forceinline__ int piece_at(int row, int piece) { return row * kSlab + ((piece ^ ((row ^ row >> 2) & 7)) << 2); }
+// A slab: adds what the formula adds and writes it, a warp eight rows, 128 bytes of the parts of a row in an access (a warp that has the 32 rows
+// that it takes out of tensor memory touches 32 lines in every access).  Columns are written as rows where a result lies turned and, of
+// symmetric matrices, what is below their diagonal blocks of 32 x 32.  (Those are written as they come: two results that mirror one
+// another have the same terms.)  Rows of parts are padded to eight values, and what is written there nobody reads.
+template <int PHASE>
+struct Slab {
+  static constexpr bool kSymmetric = PHASE == kGram || PHASE == kSquare;
+  int r, c;  // the lane's first row and column of eight; its second row is four behind
+  uint4 hi[2], lo[2];
+  __device__ __forceinline__ Slab(int row, int col, int warp, int lane) : r(row + warp * 8 + (lane >> 3)), c(col + (lane & 7) * 8) {}
+  __device__ __forceinline__ bool in(const Item& q, int k) const {
+    return r + 4 * k < q.m && c < (kSymmetric ? q.m : q.n) && (!kSymmetric || (c & ~31) <= (r & ~31));  // both rows are in one block of 32
   }
-}
-// Eight values of row r, columns c .. c + 7, of a symmetric matrix [m][m], of which those up to the diagonal are to be written, here and mirrored.
-// The lanes of the warp have 32 rows one after the other.
-__device__ __forceinline__ void write_symmetric(uint16_t* p, int64_t plane, int ld, int m, int r, int c, const float (&v)[8]) {
-  if (r >= m) return;
-  uint32_t hi[4], lo[4];
+  __device__ __forceinline__ void fetch(const Item& q, int from) {
+    if (PHASE == kGram) return;
+    const int ld = kSymmetric ? q.ldm : q.ldx;
+    const uint16_t* more = (PHASE == kSquare ? q.g : (from ? q.x[1] : q.x[0])) + (int64_t)r * ld + c;
+    const int64_t plane = (int64_t)q.m * ld;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) split2(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
-  uint16_t* at = p + (int64_t)r * ld + c;
-  const bool whole = c + 7 <= r;
-  if (whole) {
-    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(at + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint16_t h = (uint16_t)(hi[k / 2] >> (k & 1) * 16), l = (uint16_t)(lo[k / 2] >> (k & 1) * 16);
-    if (!whole && c + k <= r) {
-      at[k] = h;
-      at[k + plane] = l;
+    for (int k = 0; k < 2; ++k) {
+      hi[k] = lo[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (in(q, k)) {
+        hi[k] = __ldcg(reinterpret_cast<const uint4*>(more + (int64_t)4 * k * ld));  // written by other SMs meanwhile
+        lo[k] = __ldcg(reinterpret_cast<const uint4*>(more + (int64_t)4 * k * ld + plane));
+      }
     }
-    if (c + k < r) {
-      uint16_t* mirror = p + (int64_t)(c + k) * ld + r;
-      mirror[0] = h;
-      mirror[plane] = l;
+  }
+  // What is added has been fetched; the sums are in the slab.  row0, col0: of the slab.
+  __device__ __forceinline__ void rows(const Item& q, int from, float* slab, int row0) {
+    const int ld = kSymmetric ? q.ldm : q.ldx;
+    uint16_t* to = (PHASE == kGram ? q.g : (PHASE == kSquare ? q.s : (from ? q.x[0] : q.x[1]))) + (int64_t)r * ld + c;
+    const int64_t plane = (int64_t)q.m * ld;
+    const bool turned = PHASE == kResult ? q.tall : kSymmetric;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int y = r + 4 * k - row0, piece = (threadIdx.x & 7) * 2;
+      float4* at[2] = {reinterpret_cast<float4*>(slab + piece_at(y, piece)), reinterpret_cast<float4*>(slab + piece_at(y, piece + 1))};
+      const float4 s0 = *at[0], s1 = *at[1];
+      float v[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+      constexpr float f = (PHASE == kSquare ? kC : 1.f) / (kScale * kScale), g = PHASE == kSquare ? kB : kA;
+      const uint32_t hs[4] = {hi[k].x, hi[k].y, hi[k].z, hi[k].w}, ls[4] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] *= f;
+        v[2 * j + 1] *= f;
+        if (PHASE != kGram) {
+          const float2 w = join2(hs[j], ls[j]);
+          v[2 * j] += g * w.x;
+          v[2 * j + 1] += g * w.y;
+        }
+      }
+      if (turned) {
+        *at[0] = make_float4(v[0], v[1], v[2], v[3]);
+        *at[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      if (PHASE == kResult) {
+        if (!turned && in(q, k)) {
+          float* o = q.out + (int64_t)(r + 4 * k) * q.n + c;
+          put(q, o, make_float4(v[0], v[1], v[2], v[3]), q.n - c);
+          put(q, o + 4, make_float4(v[4], v[5], v[6], v[7]), q.n - c - 4);
+        }
+      } else if (in(q, k)) {
+        uint4 h, l;
+        split2(v[0], v[1], h.x, l.x);
+        split2(v[2], v[3], h.y, l.y);
+        split2(v[4], v[5], h.z, l.z);
+        split2(v[6], v[7], h.w, l.w);
+        *reinterpret_cast<uint4*>(to + (int64_t)4 * k * ld) = h;
+        *reinterpret_cast<uint4*>(to + (int64_t)4 * k * ld + plane) = l;
+      }
+    }
+  }
+  // A warp writes four columns as rows, a lane four values of each.
+  __device__ __forceinline__ void columns(const Item& q, const float* slab, int row0, int col0, int warp, int lane) {
+    const int y = lane * 4, first = row0 + y, left = q.m - first, width = kSymmetric ? q.m : q.n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int x = warp * 4 + k, col = col0 + x;
+      if (left <= 0 || col >= width || (kSymmetric && (col & ~31) >= (first & ~31))) continue;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = slab[piece_at(y + j, x >> 2) + (x & 3)];
+      if (kSymmetric) {
+        uint16_t* o = (PHASE == kGram ? q.g : q.s) + (int64_t)col * q.ldm + first;
+        uint2 h, l;
+        split2(v[0], v[1], h.x, l.x);
+        split2(v[2], v[3], h.y, l.y);
+        *reinterpret_cast<uint2*>(o) = h;
+        *reinterpret_cast<uint2*>(o + (int64_t)q.m * q.ldm) = l;
+      } else {
+        put(q, q.out + (int64_t)col * q.m + first, make_float4(v[0], v[1], v[2], v[3]), left);
+      }
+    }
+  }
+  // `left` of four results, none or less too
+  static __device__ __forceinline__ void put(const Item& q, float* o, const float4& w, int left) {
+    if (left <= 0) return;
+    const float keep = q.keep, step = q.step;
+    const bool update = q.update;
+    if (q.vec) {
+      float4 v = w;
+      if (update) {
+        const float4 old = *reinterpret_cast<const float4*>(o);
+        v = make_float4(keep * old.x - step * w.x, keep * old.y - step * w.y, keep * old.z - step * w.z, keep * old.w - step * w.w);
+      }
+      *reinterpret_cast<float4*>(o) = v;
+      return;
+    }
+    const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) o[j] = update ? keep * o[j] - step * v[j] : v[j];
+  }
+};
+
+// What a warp that finishes results keeps from tile to tile.
+struct Accumulators {
+  uint32_t sums, full, empty;  // tensor memory; barriers, of the first of two
+  uint32_t chunks;             // so far
+  bool ok;
+  volatile int *abort, *drawn;
+  float* slab;
+  int quad, group, lane, rank;
+};
+template <int PHASE, int W, bool PAIR>
+__device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc, int from) {
+  using M = Layout<W, PAIR>;
+  constexpr int cols = M::cols;
+  constexpr int phase = PHASE == kResult ? kApply : PHASE;
+  const int items = p.items[phase];
+  for (int i = blockIdx.x >> PAIR; i < items; i += gridDim.x >> PAIR) {  // to the end also if a wait has run out: the warps meet at barriers
+    const Tile t = tile_of<W, PAIR>(p, phase, i);
+    const int splits = p.item[t.q].splits[phase];
+    const Item q = p.item[t.q];  // of its own: what is left in the parameters is read again after every store
+    const int row0 = t.row + acc.rank * kTileM, warp = threadIdx.x >> 5, width = PHASE == kGram || PHASE == kSquare ? q.m : q.n;
+    constexpr bool early = W == 64;  // what is added is on its way during the product: elsewhere there are no registers for it
+    Slab<PHASE> slab(row0, t.col, warp, acc.lane);
+    if (early) slab.fetch(q, from);
+    const int chunk = chunk_of<W>(phase == kGram ? q.n : q.m), chunks = (t.k1 - t.k0 + chunk - 1) / chunk;
+    float sum[cols];
+#pragma unroll
+    for (int j = 0; j < cols; ++j) sum[j] = 0.f;
+    for (int ch = 0; ch < chunks && acc.ok; ++ch, ++acc.chunks) {
+      const uint32_t second = acc.chunks & 1;
+      acc.ok = __all_sync(0xffffffffu, parts::wait(acc.full + 8 * second, acc.chunks >> 1 & 1, p.status, 96, acc.abort));
+      if (!acc.ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < cols; c += 16) {
+        uint32_t v[16];
+        tmem_ld16_nowait(acc.sums + kSecond * second + c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(v[j]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (acc.lane == 0) arrive_first<PAIR>(acc.empty + 8 * second);
+    }
+    if (splits > 1) {
+      const int64_t size = (int64_t)W * kTileM;
+      float* mine = p.sums + (int64_t)((p.item[t.q].first_part[phase] + t.index * splits << PAIR) + acc.rank * splits) * size + (int64_t)acc.group * cols * kTileM + acc.quad * 32 + acc.lane;
+#pragma unroll
+      for (int j = 0; j < cols; ++j) __stcg(mine + t.split * size + j * kTileM, sum[j]);
+      __threadfence();
+      asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+      if (threadIdx.x == 0) {
+        unsigned* ticket = p.tickets + (p.item[t.q].first_ticket[phase] + t.index << PAIR) + acc.rank;
+        const int d = (int)atomicAdd(ticket, 1u);
+        if (d == splits - 1) *ticket = 0;
+        *acc.drawn = d;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+      const bool mine_to_finish = *acc.drawn == splits - 1;
+      asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");  // `drawn` has been read
+      if (!mine_to_finish) continue;
+      __threadfence();
+#pragma unroll
+      for (int j = 0; j < cols; ++j) sum[j] = 0.f;
+      for (int o = 0; o < splits; ++o)
+#pragma unroll
+        for (int j = 0; j < cols; ++j) sum[j] += __ldcg(mine + o * size + j * kTileM);
+    }
+#pragma unroll 1
+    for (int k = 0; k < W / kSlab; ++k) {
+      const int col0 = t.col + k * kSlab;
+      if (row0 >= q.m || col0 >= width || (Slab<PHASE>::kSymmetric && col0 >= row0 + kTileM)) break;  // the same for all warps
+      if (!early || k > 0) {
+        slab = Slab<PHASE>(row0, col0, warp, acc.lane);
+        slab.fetch(q, from);
+      }
+      if (acc.group * cols / kSlab == k) {
+#pragma unroll
+        for (int j = 0; j < cols; j += 4)
+          *reinterpret_cast<float4*>(acc.slab + piece_at(acc.quad * 32 + acc.lane, (acc.group * cols % kSlab + j) / 4)) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+      slab.rows(q, from, acc.slab, row0);
+      if (Slab<PHASE>::kSymmetric || (PHASE == kResult && q.tall)) {
+        asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+        slab.columns(q, acc.slab, row0, col0, warp, acc.lane);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
     }
   }
 }
 
-// Roles of a CTA, one per SM, that walks over tiles of 128 x W: a TMA warp some K-blocks of 64 ahead, an MMA warp, eight warps that empty the
-// accumulators into registers and write the result.  Where the tiles are fewer than the SMs, several CTAs share a tile's reduction: each leaves its
-// sums in memory, and the one that draws the last ticket adds them up in their order.  A K-block takes 12 MMAs; for W = 128 what crosses the
-// shared memory bounds them (107 cycles each instead of 64), for W = 256 it is 160 instead of 128.  Every wait is bounded; on expiry the kernel records
+// All products of all steps.  Roles of a CTA, one per SM, that walks over tiles: a TMA warp some K-blocks of 64 ahead, an MMA warp (of a pair's first
+// CTA), and warps that empty the accumulators into registers and write the result, 16 of them where a tile's latency counts.  Where the
+// tiles are fewer than the SMs, several CTAs share a tile's reduction: each leaves its sums in memory, and the one that draws the last ticket
+// adds them up in their order.  A K-block takes 12 MMAs.  What bounds large products otherwise is what all SMs together bring in from the L2 cache
+// (some 37 bytes a cycle and SM): a pair with W = 256 takes 64 KB a K-block and CTA for 128 x 256 results, one CTA alone would take 96.
+// Between two products a block's warps count the block as done when they have written their results, and its TMA warp waits for all blocks
+// before it brings in what the next product reads and lets the block's others go on.  Every wait is bounded; on expiry the kernel records
 // a code in the status word, raises a flag that all other waits poll, lets its own copies land, frees tensor memory and returns.
-template <int PHASE, int W>
-__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
-  RT_PDL_ENTRY();
-  using M = Smem<W>;
+template <int W, bool PAIR>
+__global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_kernel(const __grid_constant__ Product p) {
+  using M = Layout<W, PAIR>;
   constexpr int kStages = M::stages;
-  extern __shared__ char smem_raw[];
-  __shared__ volatile int abort_flag;
-  __shared__ int drawn;
-  const uint32_t raw_base = smem_u32(smem_raw), base = (raw_base + 1023) & ~1023u;
-  char* smem = smem_raw + (base - raw_base);
+  extern __shared__ __align__(1024) char smem[];  // and none besides: it starts where shared memory does
+  const uint32_t base = smem_u32(smem);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int rank = PAIR ? blockIdx.x & 1 : 0, unit = blockIdx.x >> PAIR, units = gridDim.x >> PAIR;
   const uint32_t bars = base + M::bars;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 8 * (kStages + i); };
-  const uint32_t acc_full = bars + 16 * kStages, acc_empty = acc_full + 8, cross_empty = acc_full + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + M::bars + (2 * kStages + 3) * 8);
+  const uint32_t acc_full = bars + 16 * kStages, acc_empty = acc_full + 16, go = acc_full + 32;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + M::bars + (2 * kStages + 5) * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    *abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full(i), 1);
       mbar_init(empty(i), 1);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, kEpilogueWarps);
-    mbar_init(cross_empty, kEpilogueWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, M::warps << PAIR);
+    }
+    mbar_init(go, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == M::mma) allocate<PAIR>(smem_u32(tmem_slot));
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cg::this_cluster().sync();  // the barriers, too, are there
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   bool ok = true;
 
-  if (warp == kTmaWarp) {
+  if (warp == M::tma) {
     if (lane == 0) {
-      asm volatile("fence.proxy.async.global;" ::: "memory");  // the parts were written by ordinary stores
       int it = 0;
-      for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-        const Tile t = tile_of<PHASE, W>(p, i);
-        const CUtensorMap* map_a = PHASE == kGram ? &p.x[p.from][t.q] : (PHASE == kSquare ? &p.g[t.q] : &p.s[t.q]);
-        const CUtensorMap* map_b = PHASE == kSquare ? &p.g[t.q] : &p.x[p.from][t.q];
-        const int boxes = (min(W, (PHASE == kApply ? p.item[t.q].n : p.item[t.q].m) - t.col) + 63) / 64;
-        for (int kb = t.k0; kb < t.k1 && ok; ++kb, ++it) {
-          const int st = it % kStages;
-          if (it >= kStages) ok = parts::wait(empty(st), (it / kStages - 1) & 1, p.status, 91, &abort_flag);
-          if (!ok) break;
-          const uint32_t dst = base + st * M::stage;
-          mbar_expect_tx(full(st), (4 + 2 * boxes) * kBox);
-          for (int z = 0; z < 2; ++z) {
-            for (int j = 0; j < 2; ++j) load_3d(dst + (2 * z + j) * kBox, map_a, kb * kBlockK, t.row + j * 64, z, full(st));
-            for (int j = 0; j < boxes; ++j) {
-              const int n = t.col + j * 64;
-              load_3d(dst + (4 + z * (W / 64) + j) * kBox, map_b, PHASE == kApply ? n : kb * kBlockK, PHASE == kApply ? kb * kBlockK : n, z, full(st));
+      for (int product = 0; product < 3 * p.steps && ok; ++product) {
+        const int phase = product % 3, from = product / 3 & 1, items = p.items[phase];
+        Tile t = tile_of<W, PAIR>(p, phase, unit);  // before the wait: a thousand cycles
+        if (product > 0) {
+          const unsigned all = gridDim.x * (unsigned)product;
+          unsigned there = 0;
+          for (uint32_t k = 0; k < kSpinLimit && there < all && !*abort_flag; ++k)
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.arrived) : "memory");
+          if (there < all) {
+            if (!*abort_flag) record_status(p.status, 97);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          mbar_arrive(go);
+        }
+        asm volatile("fence.proxy.async.global;" ::: "memory");  // the parts were written by ordinary stores
+        for (int i = unit; i < items && ok; i += units) {
+          if (i != unit) t = tile_of<W, PAIR>(p, phase, i);
+          const CUtensorMap* map_a = phase == kGram ? &p.x_left[from][t.q] : (phase == kSquare ? &p.g_left[t.q] : &p.s_left[t.q]);
+          const CUtensorMap* map_b = phase == kGram ? &p.x_right[from][t.q] : (phase == kSquare ? &p.g_right[t.q] : &p.x_apply[from][t.q]);
+          for (int kb = t.k0; kb < t.k1 && ok; ++kb, ++it) {
+            const int st = it % kStages;
+            if (it >= kStages) ok = parts::wait(empty(st), (it / kStages - 1) & 1, p.status, 91, abort_flag);
+            if (!ok) break;
+            const uint32_t dst = base + st * M::stage;
+            if (rank == 0) mbar_expect_tx(full(st), M::stage << PAIR);
+            load_3d<PAIR>(dst, map_a, kb * kBlockK, t.row + rank * kTileM, 0, full(st));
+            const int col = t.col + rank * M::right;
+            if (phase == kApply) {
+#pragma unroll
+              for (int j = 0; j < M::right / 64; ++j) load_3d<PAIR>(dst + (4 + 2 * j) * kBox, map_b, col + j * 64, kb * kBlockK, 0, full(st));
+            } else {
+              load_3d<PAIR>(dst + 4 * kBox, map_b, kb * kBlockK, col, 0, full(st));
             }
           }
         }
       }
       // copies that nobody has waited for must have landed before the CTA may leave
-      if (!ok)
+      if (!ok && rank == 0)
         for (int i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait(full(i % kStages), (i / kStages) & 1, p.status, 92);
     }
-  } else if (warp == kMmaWarp) {
-    // descriptors as in parts_common.cuh: groups of 8 rows (of 8 K) 1024 bytes apart, 128-byte swizzle; where the columns lie side by side instead of
-    // the reduction, groups of 64 columns a box apart
+  } else if (warp == M::mma) {
+    if (rank == 0) {
+    // Descriptors as in parts_common.cuh: groups of 8 rows (of 8 K) 1024 bytes apart, 128-byte swizzle; where the columns lie side by side instead of
+    // the reduction, groups of 64 columns, both planes of them, 2 * kBox apart.
     constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    constexpr uint32_t lbo = (kBox >> 4) << 16, slot_a = 32 >> 4, slot_b = PHASE == kApply ? 2048 >> 4 : 32 >> 4;
-    constexpr uint32_t idesc0 = (1u << 4) | (uint32_t)(PHASE == kApply) << 16 | (uint32_t)(kTileM >> 4) << 24;
-    int it = 0, chunks = 0, tiles = 0;
-    for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-      const Tile t = tile_of<PHASE, W>(p, i);
-      const int width = (PHASE == kApply ? p.item[t.q].n : p.item[t.q].m) - t.col, depth = PHASE == kGram ? p.item[t.q].n : p.item[t.q].m;
-      const uint32_t idesc = idesc0 | (uint32_t)(min(W, (width + 15) & ~15) >> 3) << 17;
-      for (int kb = t.k0, in_chunk = 0; kb < t.k1 && ok; ++kb, ++it) {
-        const int st = it % kStages;
-        const bool first = in_chunk == 0, last = ++in_chunk == p.chunk || kb + 1 == t.k1;
-        if (last) in_chunk = 0;
-        ok = parts::wait(full(st), (it / kStages) & 1, p.status, 93, &abort_flag);
-        if (ok && kb == t.k0 && tiles > 0) ok = parts::wait(cross_empty, (tiles - 1) & 1, p.status, 94, &abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t a = ((base + st * M::stage) >> 4 & 0x3FFF) | lbo, b = ((base + st * M::stage + 4 * kBox) >> 4 & 0x3FFF) | lbo;
-        const uint32_t a_lo = a + (2 * kBox >> 4), b_lo = b + (W / 64 * kBox >> 4), cross = tmem + kCross;
-        const int slots = min(kBlockK, depth - kb * kBlockK + 15) / 16;  // what is behind the reduction is zeros
-        for (int k = 0; k < slots; ++k) {
-          parts::mma(cross, a + k * slot_a, desc_hi, b_lo + k * slot_b, desc_hi, idesc, kb > t.k0 || k > 0);
-          parts::mma(cross, a_lo + k * slot_a, desc_hi, b + k * slot_b, desc_hi, idesc, 1);
-        }
-        if (first && chunks > 0) {
-          ok = __all_sync(0xffffffffu, parts::wait(acc_empty, (chunks - 1) & 1, p.status, 95, &abort_flag));
+    constexpr uint32_t lbo = (2 * kBox >> 4) << 16, slot_a = 32 >> 4;  // mma_block has the latter as 2
+    int it = 0;
+    uint32_t chunks = 0;
+    for (int product = 0; product < 3 * p.steps && ok; ++product) {
+      const int phase = product % 3, items = p.items[phase];
+      const uint32_t slot_b = phase == kApply ? 2048 >> 4 : 32 >> 4;
+      const uint32_t idesc = (1u << 4) | (uint32_t)(phase == kApply) << 16 | (uint32_t)(M::rows >> 4) << 24 | (uint32_t)(W >> 3) << 17;
+      for (int i = unit; i < items && ok; i += units) {
+        const Tile t = tile_of<W, PAIR>(p, phase, i);
+        const int depth = phase == kGram ? p.item[t.q].n : p.item[t.q].m, chunk = chunk_of<W>(depth);
+        for (int kb = t.k0, in_chunk = 0; kb < t.k1 && ok; ++kb, ++it) {
+          const int st = it % kStages;
+          const bool first = in_chunk == 0, last = ++in_chunk == chunk || kb + 1 == t.k1;
+          if (last) in_chunk = 0;
+          const uint32_t a = ((base + st * M::stage) >> 4 & 0x3FFF) | lbo, b = ((base + st * M::stage + 4 * kBox) >> 4 & 0x3FFF) | lbo;
+          const uint32_t a_lo = a + (2 * kBox >> 4), b_lo = b + ((phase == kApply ? 1 : M::right / 64) * kBox >> 4), second = chunks & 1;
+          const uint32_t d = tmem + kSecond * second, more = !first;
+          const int slots = min(kBlockK, depth - kb * kBlockK + 15) / 16;  // what is behind the reduction is zeros
+          ok = parts::wait(full(st), (it / kStages) & 1, p.status, 93, abort_flag);
+          if (ok && first && chunks > 1) ok = parts::wait(acc_empty + 8 * second, ((chunks >> 1) - 1) & 1, p.status, 94, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-        }
-        for (int k = 0; k < slots; ++k) parts::mma(tmem, a + k * slot_a, desc_hi, b + k * slot_b, desc_hi, idesc, !first || k > 0);
-        umma_commit_elect(empty(st));
-        if (last) {
-          umma_commit_elect(acc_full);
-          ++chunks;
-        }
-      }
-      ++tiles;
-    }
-  } else {
-    constexpr int half = W / 2;  // columns of a group of four warps
-    const int quad = warp & 3, group = warp >> 2;
-    const uint32_t d = tmem + ((uint32_t)(quad * 32) << 16) + group * half;
-    uint32_t parity = 0;
-    for (int i = blockIdx.x; i < p.items; i += gridDim.x) {  // to the end also if a wait has run out: the warps meet at barriers
-      const Tile t = tile_of<PHASE, W>(p, i);
-      const Item& q = p.item[t.q];
-      const int chunks = (t.k1 - t.k0 + p.chunk - 1) / p.chunk;
-      float sum[half];
-#pragma unroll
-      for (int j = 0; j < half; ++j) sum[j] = 0.f;
-      for (int ch = 0; ch < chunks && ok; ++ch) {
-        ok = __all_sync(0xffffffffu, parts::wait(acc_full, parity, p.status, 96, &abort_flag));
-        if (!ok) break;
-        parity ^= 1;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < half; c += 32) {
-          float v[32];
-          tmem_ld32(d + c, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sum[c + j] += v[j];
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty);
-      }
-      if (ok) {
-#pragma unroll
-        for (int c = 0; c < half; c += 32) {
-          float v[32];
-          tmem_ld32(d + kCross + c, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sum[c + j] = (sum[c + j] + v[j] * (1.f / kLow)) * (1.f / (kScale * kScale));
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(cross_empty);
-      }
-
-      if (q.splits > 1) {
-        const int64_t size = (int64_t)W * kTileM;
-        float* mine = p.sums + (int64_t)(q.first_part + t.index * q.splits) * size + (int64_t)group * half * kTileM + quad * 32 + lane;
-#pragma unroll
-        for (int j = 0; j < half; ++j) __stcg(mine + t.split * size + j * kTileM, sum[j]);
-        __threadfence();
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (threadIdx.x == 0) {
-          unsigned* ticket = p.tickets + q.first_ticket + t.index;
-          drawn = (int)atomicAdd(ticket, 1u);
-          if (drawn == q.splits - 1) *ticket = 0;
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const bool mine_to_finish = drawn == q.splits - 1;
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // `drawn` has been read
-        if (!mine_to_finish) continue;
-        __threadfence();
-#pragma unroll
-        for (int j = 0; j < half; ++j) sum[j] = 0.f;
-        for (int o = 0; o < q.splits; ++o)
-#pragma unroll
-          for (int j = 0; j < half; ++j) sum[j] += __ldcg(mine + o * size + j * kTileM);
-      }
-      if (!ok) continue;
-
-      const int r = t.row + quad * 32 + lane;
-#pragma unroll
-      for (int c0 = 0; c0 < half; c0 += 8) {
-        const int c = t.col + group * half + c0;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = sum[c0 + j];
-        if (PHASE == kGram) {
-          if (c < q.m) write_symmetric(q.g, (int64_t)q.m * q.ldm, q.ldm, q.m, r, c, v);
-        } else if (PHASE == kSquare) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= kC;
-          if (c < q.m && r < q.m) add_parts(v, q.g + (int64_t)r * q.ldm + c, (int64_t)q.m * q.ldm, kB);
-          if (c < q.m) write_symmetric(q.s, (int64_t)q.m * q.ldm, q.ldm, q.m, r, c, v);
-        } else if (c < q.n && r < q.m) {
-          const int64_t plane = (int64_t)q.m * q.ldx, at = (int64_t)r * q.ldx + c;
-          add_parts(v, q.x[p.from] + at, plane, kA);
-          if (!p.last) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split2(v[2 * j], v[2 * j + 1], hi[j], lo[j]);
-            uint16_t* to = q.x[p.from ^ 1] + at;  // rows are padded to eight values
-            *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(to + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (slots == kBlockK / 16) {
+            mma_block<PAIR>(d, a, a_lo, b, b_lo, slot_b, desc_hi, idesc, more);
           } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (c + j >= q.n) break;
-              float* o = q.out + (q.tall ? (int64_t)(c + j) * q.m + r : (int64_t)r * q.n + c + j);
-              *o = q.update ? q.keep * *o - q.step * v[j] : v[j];
+            for (int k = 0; k < slots; ++k) {
+              mma_one<PAIR>(d, a + k * slot_a, b_lo + k * slot_b, desc_hi, idesc, more | (uint32_t)(k > 0));
+              mma_one<PAIR>(d, a_lo + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
             }
+            for (int k = 0; k < slots; ++k) mma_one<PAIR>(d, a + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
+          }
+          commit<PAIR>(empty(st));
+          if (last) {
+            commit<PAIR>(acc_full + 8 * second);
+            ++chunks;
           }
         }
       }
     }
+    }
+  } else {
+    Accumulators acc;
+    acc.rank = rank;
+    acc.quad = warp & 3;
+    acc.group = warp >> 2;
+    acc.lane = lane;
+    acc.sums = tmem + ((uint32_t)(acc.quad * 32) << 16) + acc.group * M::cols;
+    acc.full = acc_full;
+    acc.empty = acc_empty;
+    acc.chunks = 0;
+    acc.ok = true;
+    acc.abort = abort_flag;
+    acc.drawn = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    acc.slab = reinterpret_cast<float*>(smem + M::slab);
+    for (int step = 0; step < p.steps; ++step) {
+#pragma unroll 1
+      for (int phase = 0; phase < 3; ++phase) {
+        const int product = 3 * step + phase;
+        if (product > 0 && acc.ok) acc.ok = __all_sync(0xffffffffu, parts::wait(go, (product - 1) & 1, p.status, 98, abort_flag));
+        if (phase == kGram) finish_tiles<kGram, W, PAIR>(p, acc, step & 1);
+        else if (phase == kSquare) finish_tiles<kSquare, W, PAIR>(p, acc, step & 1);
+        else if (step + 1 < p.steps) finish_tiles<kApply, W, PAIR>(p, acc, step & 1);
+        else finish_tiles<kResult, W, PAIR>(p, acc, step & 1);
+        if (product + 1 == 3 * p.steps) break;
+        asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+        if (threadIdx.x == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.arrived) : "memory");
+      }
+    }
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == kMmaWarp) {
+  if (PAIR) cg::this_cluster().sync();  // neither leaves while the other still uses its memory
+  else __syncthreads();
+  if (warp == M::mma) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    release<PAIR>(tmem);
   }
 }
 
@@ -456,11 +799,6 @@ struct Parts {
   int count;
   unsigned *tickets, tickets_end;
 };
-__device__ __forceinline__ float one_over_norm(const double* __restrict__ sums) {
-  double sum = 0.0;
-  for (int b = 0; b < kNormBlocks; ++b) sum += __ldg(sums + b);
-  return (float)(1.0 / (sqrt(sum) + kEpsilon));
-}
 __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__ Parts p) {
   RT_PDL_ENTRY();
   __shared__ float tile[64][65];
@@ -472,7 +810,10 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   const int64_t rows = p.rows[q], cols = p.cols[q];
   const unsigned local = blockIdx.x - p.first[q], tiles_c = (unsigned)((cols + 63) / 64);
   const int64_t r0 = (int64_t)(local / tiles_c) * 64, c0 = (int64_t)(local % tiles_c) * 64;
-  if (threadIdx.x == 0) by = one_over_norm(p.sums[q]);
+  if (threadIdx.x < 32) {
+    const float f = one_over_norm(p.sums[q]);
+    if (threadIdx.x == 0) by = f;
+  }
   const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
   float v[16];
 #pragma unroll
@@ -504,55 +845,88 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   (void)n;
 }
 
-// [2 planes][rows][cols] halves, rows ld apart, boxes of 64 x 64 of one plane, zeros outside.
-bool map_planes(CUtensorMap* map, uint16_t* t, int64_t cols, int64_t rows, int64_t ld) {
+// [2 planes][rows][cols] halves, rows ld apart, boxes of 64 columns and `height` rows of both planes, zeros outside.
+bool map_planes(CUtensorMap* map, uint16_t* t, int64_t cols, int64_t rows, int64_t ld, int height) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 2}, strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(ld * rows) * 2};
-  const cuuint32_t box[3] = {64, 64, 1}, one[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)height, 2}, one[3] = {1, 1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, t, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a product's tiles are laid out over the SMs: their width, and into how many parts the reduction of each matrix's tiles is split.
+// How the tiles are laid out over the SMs: their width (64: of one CTA, 128 and 256: of a pair), and into how many parts the reduction of each
+// matrix's tiles is split, by product.
 struct Plan {
-  int width, splits[kGroup];
+  int width, splits[3][kGroup];
 };
+int rows_of_tile(int width) { return width == 64 ? kTileM : 2 * kTileM; }
 int64_t tiles_of(int phase, int width, int64_t m, int64_t n) {
-  const int64_t rows = (m + kTileM - 1) / kTileM;
+  const int64_t height = rows_of_tile(width), rows = (m + height - 1) / height;
   if (phase == kApply) return rows * ((n + width - 1) / width);
-  return width == kTileM ? rows * (rows + 1) / 2 : (rows / 2) * (rows / 2 + 1) + (rows % 2) * (rows / 2 + 1);
+  if (width == height) return rows * (rows + 1) / 2;
+  const int64_t all = rows * (rows + 1);
+  return (rows - 1) * height + width >= m ? all - 1 : all;  // the last one has no columns
 }
-// In units of a K-block of a tile of 128 x 128, 0.68 us; one of 128 x 256 takes 1.5 of them, sharing a reduction about 5.
-Plan plan_product(const rt_ctx* ctx, int phase, int count, const Item* items) {
+// In cycles, as measured: a K-block, what a tile takes besides, what sharing a reduction takes.  Microseconds with 64, 128 and 256 columns: 512 x 512 158,
+// 204 and 339; 1024 x 1024 218, 288 and 447; 2000 x 2600 1093, 786 and 911; with 128 and 256 columns
+// 4096 x 4096 4480 and 3585.
+Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
   Plan best{};
   double least = 1e300;
-  for (int width = 128; width <= 256; width *= 2)
-    for (int most = 64; most >= 1; most /= 2) {  // K-blocks of a CTA at most, where that needs several CTAs
-      Plan p{};
-      p.width = width;
-      double work = 0, longest = 0;
-      for (int q = 0; q < count; ++q) {
-        const int blocks = ((phase == kGram ? items[q].n : items[q].m) + kBlockK - 1) / kBlockK;
-        p.splits[q] = most == 64 || width == 256 ? 1 : (blocks + most - 1) / most;
-        const double one = (width == 256 ? 1.5 : 1.0) * ((blocks + p.splits[q] - 1) / p.splits[q]) + (p.splits[q] > 1 ? 5 + 0.5 * p.splits[q] : 0);
-        work += one * (double)tiles_of(phase, width, items[q].m, items[q].n) * p.splits[q];
-        longest = std::max(longest, one);
+  for (int width = 64; width <= 256; width *= 2) {
+    Plan p{};
+    p.width = width;
+    double sum = 0;
+    const double block = width == 256 ? 1550 : (width == 128 ? 1000 : 1050), rest = width == 256 ? 22000 : (width == 128 ? 11000 : 4500);
+    const int units = width == 64 ? ctx->sm_count : ctx->sm_count / 2;
+    for (int phase = 0; phase < 3; ++phase) {
+      double least_here = 1e300;
+      for (int most = 64; most >= 1; most /= 2) {  // K-blocks of a tile at most, where that needs it split
+        int splits[kGroup];
+        double work = 0, longest = 0;
+        for (int q = 0; q < count; ++q) {
+          const int blocks = ((phase == kGram ? items[q].n : items[q].m) + kBlockK - 1) / kBlockK;
+          splits[q] = most == 64 ? 1 : (blocks + most - 1) / most;
+          const double one = block * ((blocks + splits[q] - 1) / splits[q]) + rest + (splits[q] > 1 ? (4600 + 400 * splits[q]) * (width / 64) : 0);
+          work += one * (double)tiles_of(phase, width, items[q].m, items[q].n) * splits[q];
+          longest = std::max(longest, one);
+        }
+        const double time = std::max(longest, work / units) + 0.5 * longest;  // the last tiles do not all end at once
+        if (time < least_here) {
+          least_here = time;
+          std::copy(splits, splits + count, p.splits[phase]);
+        }
       }
-      const double time = std::max(longest, work / ctx->sm_count) + 0.5 * longest;  // the last tiles do not all end at once
-      if (time < least) {
-        least = time;
-        best = p;
-      }
-      if (width == 256) break;
+      sum += least_here;
     }
+    if (sum < least) {
+      least = sum;
+      best = p;
+    }
+  }
   return best;
 }
-template <int PHASE, int W>
-rt_status launch_product(rt_ctx* ctx, const Product& p) {
+template <int W, bool PAIR>
+rt_status launch_products(rt_ctx* ctx, const Product& p) {
+  using M = Layout<W, PAIR>;
   static RtDeviceOnce once;
-  RT_CUDA(ctx, once([] { return cudaFuncSetAttribute(product_kernel<PHASE, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<W>::bytes); }));
-  rt_launch(ctx, product_kernel<PHASE, W>, p.items < ctx->sm_count ? p.items : ctx->sm_count, kProductThreads, Smem<W>::bytes, p);
+  RT_CUDA(ctx, once([] { return cudaFuncSetAttribute(newton_schulz_kernel<W, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)M::bytes); }));
+  const int items = std::max(p.items[0], std::max(p.items[1], p.items[2])), units = ctx->sm_count >> PAIR;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = (unsigned)std::min(items, units) << PAIR;
+  cfg.blockDim = M::threads;
+  cfg.dynamicSmemBytes = M::bytes;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  RT_CUDA(ctx, cudaLaunchKernelEx(&cfg, newton_schulz_kernel<W, PAIR>, p));
   RT_LAUNCHED(ctx);
   return RT_OK;
 }
@@ -575,30 +949,41 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     i.out = list[q].out;
     i.tall = list[q].rows > list[q].cols;
     i.update = list[q].update;
+    i.vec = list[q].cols % 4 == 0 && rt_aligned16(i.out);
     i.keep = list[q].keep;
     i.step = list[q].step;
   }
-  Plan plans[3];
+  p.steps = steps;
+  const Plan plan = plan_products(ctx, count, p.item);
   size_t partials = 0, tickets = 0;
   for (int phase = 0; phase < 3; ++phase) {
-    plans[phase] = plan_product(ctx, phase, count, p.item);
-    size_t parts_of = 0, tickets_of = 0;
-    for (int q = 0; q < count; ++q)
-      if (plans[phase].splits[q] > 1) {
-        const size_t tiles = (size_t)tiles_of(phase, plans[phase].width, p.item[q].m, p.item[q].n);
-        parts_of += tiles * plans[phase].splits[q];
-        tickets_of += tiles;
+    int items = 0, first_part = 0, first_ticket = 0;
+    for (int q = 0; q < count; ++q) {
+      Item& i = p.item[q];
+      const int tiles = (int)tiles_of(phase, plan.width, i.m, i.n), splits = plan.splits[phase][q];
+      i.splits[phase] = splits;
+      i.first[phase] = items;
+      i.first_part[phase] = first_part;
+      i.first_ticket[phase] = first_ticket;
+      items += tiles * splits;
+      if (splits > 1) {
+        first_part += tiles * splits;
+        first_ticket += tiles;
       }
-    partials = std::max(partials, parts_of * plans[phase].width * kTileM);
-    tickets = std::max(tickets, tickets_of);
+    }
+    p.items[phase] = items;
+    partials = std::max(partials, (size_t)first_part * plan.width * rows_of_tile(plan.width));
+    tickets = std::max(tickets, (size_t)first_ticket * 2);
   }
   RtScratch work(ctx);
-  rt_status st = work.alloc(sizeof(uint16_t) * halves + sizeof(float) * partials + sizeof(double) * kNormBlocks * count + sizeof(unsigned) * tickets);
+  rt_status st = work.alloc(sizeof(uint16_t) * halves + sizeof(float) * partials + sizeof(double) * kNormBlocks * count + sizeof(unsigned) * (tickets + 1));
   if (st != RT_OK) return st;
   p.sums = reinterpret_cast<float*>(work.as<uint16_t>() + halves);
   double* squares = reinterpret_cast<double*>(p.sums + partials);
   p.tickets = reinterpret_cast<unsigned*>(squares + (size_t)kNormBlocks * count);
+  p.arrived = p.tickets + tickets;
   unsigned tiles = 0;
+  const int right = plan.width == 64 ? 64 : plan.width / 2;  // columns that a CTA brings in
   for (int q = 0; q < count; ++q) {
     Item& i = p.item[q];
     const size_t of_x = (size_t)2 * i.m * i.ldx, of_g = (size_t)2 * i.m * i.ldm;
@@ -606,8 +991,12 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     i.x[1] = i.x[0] + of_x;
     i.g = i.x[1] + of_x;
     i.s = i.g + of_g;
-    if (!map_planes(&p.x[0][q], i.x[0], i.n, i.m, i.ldx) || !map_planes(&p.x[1][q], i.x[1], i.n, i.m, i.ldx) ||
-        !map_planes(&p.g[q], i.g, i.m, i.m, i.ldm) || !map_planes(&p.s[q], i.s, i.m, i.m, i.ldm)) {
+    bool mapped = map_planes(&p.g_left[q], i.g, i.m, i.m, i.ldm, kTileM) && map_planes(&p.g_right[q], i.g, i.m, i.m, i.ldm, right) &&
+                  map_planes(&p.s_left[q], i.s, i.m, i.m, i.ldm, kTileM);
+    for (int k = 0; k < 2; ++k)
+      mapped = mapped && map_planes(&p.x_left[k][q], i.x[k], i.n, i.m, i.ldx, kTileM) && map_planes(&p.x_right[k][q], i.x[k], i.n, i.m, i.ldx, right) &&
+               map_planes(&p.x_apply[k][q], i.x[k], i.n, i.m, i.ldx, 64);
+    if (!mapped) {
       *unavailable = true;
       return RT_OK;
     }
@@ -622,42 +1011,11 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
   }
   x.first[count] = tiles;
   x.tickets = p.tickets;
-  x.tickets_end = (unsigned)tickets;
-  for (int q = 0; q < count; ++q) {
-    rt_launch(ctx, squares_kernel, kNormBlocks, kThreads, 0, list[q].u, list[q].rows * list[q].cols, squares + (size_t)kNormBlocks * q);
-    RT_LAUNCHED(ctx);
-  }
+  x.tickets_end = (unsigned)tickets + 1;  // and the count of the blocks
+  if ((st = launch_squares(ctx, list, count, squares)) != RT_OK) return st;
   rt_launch(ctx, parts_kernel, tiles, kThreads, 0, x);
   RT_LAUNCHED(ctx);
-  for (int k = 0; k < steps; ++k) {
-    p.from = k & 1;
-    p.last = k + 1 == steps;
-    for (int phase = 0; phase < 3; ++phase) {
-      int items = 0, first_part = 0, first_ticket = 0, depth = 0;
-      for (int q = 0; q < count; ++q) {
-        Item& i = p.item[q];
-        const int t = (int)tiles_of(phase, plans[phase].width, i.m, i.n);
-        i.splits = plans[phase].splits[q];
-        i.first = items;
-        i.first_part = first_part;
-        i.first_ticket = first_ticket;
-        items += t * i.splits;
-        if (i.splits > 1) {
-          first_part += t * i.splits;
-          first_ticket += t;
-        }
-        depth = std::max(depth, phase == kGram ? i.n : i.m);
-      }
-      p.items = items;
-      p.chunk = depth < 1024 ? 3 : (depth < 2048 ? 4 : 8);
-      const bool wide = plans[phase].width == 256;
-      if (phase == kGram) st = wide ? launch_product<kGram, 256>(ctx, p) : launch_product<kGram, 128>(ctx, p);
-      else if (phase == kSquare) st = wide ? launch_product<kSquare, 256>(ctx, p) : launch_product<kSquare, 128>(ctx, p);
-      else st = wide ? launch_product<kApply, 256>(ctx, p) : launch_product<kApply, 128>(ctx, p);
-      if (st != RT_OK) return st;
-    }
-  }
-  return RT_OK;
+  return plan.width == 256 ? launch_products<256, true>(ctx, p) : (plan.width == 128 ? launch_products<128, true>(ctx, p) : launch_products<64, false>(ctx, p));
 }
 
 // ---- by the framework's other products: without tensor cores, or with no steps ------------------------------------------------------------
@@ -668,8 +1026,7 @@ rt_status orthogonalize(rt_ctx* ctx, const Matrix& q, int steps) {
   if (st != RT_OK) return st;
   double* sums = work.as<double>();
   float *x = reinterpret_cast<float*>(sums + kNormBlocks), *y = x + all, *g = y + all, *s = g + m * m;
-  rt_launch(ctx, squares_kernel, kNormBlocks, kThreads, 0, q.u, all, sums);
-  RT_LAUNCHED(ctx);
+  if ((st = launch_squares(ctx, &q, 1, sums)) != RT_OK) return st;
   rt_launch(ctx, normalise_kernel, rt_grid_for(ctx, all, kThreads), kThreads, 0, q.u, q.rows, q.cols, sums, x);
   RT_LAUNCHED(ctx);
   for (int k = 0; k < steps; ++k) {
