@@ -266,6 +266,61 @@ def test_orthogonalize(capi, steps):
         as_near_as_fp32(dx.numpy(), ref.orthogonalize(x, steps), ref.orthogonalize(x, steps, np.float32))
 
 
+# Lists whose products go by pairs of CTAs, with tiles of 128 columns and of 256, among them shared reductions, tall matrices and small ones that
+# are edges only.
+LARGE = [
+    [(1501, 1603)],
+    [(12000, 513), (513, 12001), (513, 12000)],
+    [(701, 703)] * 6 + [(703, 690)] * 4 + [(3, 5), (1, 9)],
+    [(1290, 1803)] * 5 + [(1803, 1290), (7, 1), (129, 300)],
+    [(700, 20000)] * 3 + [(20001, 701)],
+    [(3001, 2999)],
+]
+
+
+def steps_on_gpu(u, dtype):
+    """Five Newton-Schulz steps; in 64 bits, or in fp32 as a plain program has them."""
+    import torch
+
+    x = torch.from_numpy(u).cuda().to(torch.float64)
+    x = (x / (x.square().sum().sqrt() + 1e-7)).to(dtype)
+    x = x.T if u.shape[0] > u.shape[1] else x
+    for _ in range(5):
+        g = x @ x.T
+        x = 3.4445 * x + (-4.7750 * g + 2.0315 * (g @ g)) @ x
+    return (x.T if u.shape[0] > u.shape[1] else x).double().cpu().numpy()
+
+
+@pytest.mark.parametrize("shapes", LARGE, ids=lambda s: f"{len(s)}x{s[0][0]}x{s[0][1]}")
+def test_muon_step_of_large_matrices(capi, shapes):
+    """With a step of one, nothing kept of the parameters and no momentum, so that the parameters are the orthogonalised gradients themselves."""
+    import torch
+
+    r = rng(35)
+    host = [matrix(r, s) for s in shapes]
+    g, zeros = [capi.to_device(x) for x in host], [np.zeros(x.size + 8, np.float32) for x in host]
+    for z in zeros:
+        z[-8:] = 7
+    p, m = ([capi.to_device(z) for z in zeros] for _ in range(2))
+    capi.call("muon_step_multi", len(shapes), pointers(p), pointers(g), pointers(m), capi.i64([s[0] for s in shapes]), capi.i64([s[1] for s in shapes]), f32(-1.0), f32(0.0),
+              0, f32(0.0), 5, f32(1.0))
+    for x, d, s in zip(host, p, shapes):
+        got = d.numpy()
+        assert np.all(got[x.size :] == 7)
+        got = got[: x.size].reshape(s) / max(1.0, s[1] / s[0]) ** 0.5
+        as_near_as_fp32(got, steps_on_gpu(x, torch.float64), steps_on_gpu(x, torch.float32))
+
+
+@pytest.mark.parametrize("steps", [1, 5])
+def test_orthogonalize_by_either_path(capi, contraction_path, steps):
+    r = rng(36)
+    for shape in ((1, 6), (65, 30), (140, 333), (700, 512)):
+        x = matrix(r, shape)
+        d, out = capi.to_device(x), capi.empty(shape)
+        capi.call("orthogonalize_list", 1, pointers([d]), capi.i64([shape[0]]), capi.i64([shape[1]]), steps, pointers([out]))
+        as_near_as_fp32(out.numpy(), ref.orthogonalize(x, steps), ref.orthogonalize(x, steps, np.float32))
+
+
 @pytest.mark.parametrize("value", [0.0, 1e-30, 1e30, np.nan, np.inf])
 def test_orthogonalize_of_special_matrices(capi, value):
     r = rng(32)
