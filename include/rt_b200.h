@@ -289,13 +289,13 @@ rt_status rt_upload_gather_rows(rt_ctx* ctx, rt_upload* up, int n_src, const flo
 /* ---- token embeddings (no counterpart in the reference, whose char-LSTM example multiplies one-hot rows with its weights:
  * examples/lstm_char_rnn_cpu.rs) --------------------------------------------------------------------------------------
  * ids: n int32 row numbers in DEVICE memory; one outside [0, rows) is padding.
- * out[i, :] = scale * table[ids[i], :] for a row-major table[rows, cols]; zeros where ids[i] is padding. */
+ * out[i, :] = scale * table[ids[i], :] for a row-major table[rows, cols]; zeros where ids[i] is padding.  Results must not overlap what is read. */
 rt_status rt_embedding(rt_ctx* ctx, const float* table, int64_t rows, int64_t cols, const int32_t* ids, int64_t n, float scale, float* out);
 /* dtable[r, :] = scale * the sum of g[i, :] over the i with ids[i] = r, which are added in a fixed order: the same inputs give the same bits.
  * With accumulate != 0 it is added to what is there, and rows without a token are neither read nor written. */
 rt_status rt_embedding_backward(rt_ctx* ctx, const float* g, const int32_t* ids, int64_t n, int64_t rows, int64_t cols, float scale, float* dtable,
                                 int accumulate);
-/* ids[i] = x[i], which holds whole numbers as floats like the results of argmax; -1 for a fraction, NaN and what int32 does not hold. */
+/* ids[i] = x[i], which holds whole numbers as floats like the results of argmax; -1 for a fraction, NaN and what int32 does not hold.  In place, too. */
 rt_status rt_token_ids(rt_ctx* ctx, const float* x, int64_t n, int32_t* ids);
 
 /* out[c] += sum over r of x[r, c] for a row-major x[rows, cols]: the gradient of a bias that already holds a gradient (a bias
@@ -349,9 +349,10 @@ rt_status rt_lstm_sequence_backward(rt_ctx* ctx, const float* saved, const float
 
 /* Gated linear recurrence over a sequence, time-major (no counterpart in the reference): a_t = sigmoid(f_t), h_t = a_t h_{t-1} + (1 - a_t) v_t.
  * f, v: [steps*batch, hidden] with rows ld floats apart: two matrices, or two column blocks of one.  h0 [batch, hidden] or NULL for zeros;
- * h [steps*batch, hidden]; with one timestep h may be h0 (the state of a model that generates, updated in place).  f = +inf keeps the state
+ * h [steps*batch, hidden]; with one timestep h may be h0 (the state of a model that generates, updated in place), or f or v if ld = hidden.  f = +inf keeps the state
  * (padding at a sequence's end), f = -inf takes v alone (a sequence's first timestep among others), if state and v are finite.
- * Backward, from h and dh = the gradient of every h_t: df, dv with rows ldd apart, dh0 [batch, hidden] or NULL. */
+ * Backward, from h and dh = the gradient of every h_t: df, dv with rows ldd apart, dh0 [batch, hidden] or NULL.  Otherwise results must not overlap
+ * what is read, nor one another. */
 rt_status rt_gated_scan(rt_ctx* ctx, const float* f, const float* v, int64_t ld, const float* h0, int64_t steps, int64_t batch, int64_t hidden, float* h);
 rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, int64_t ld, const float* h0, const float* h, const float* dh, int64_t steps,
                                  int64_t batch, int64_t hidden, float* df, float* dv, int64_t ldd, float* dh0);

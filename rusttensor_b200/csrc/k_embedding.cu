@@ -572,6 +572,7 @@ rt_status rt_token_ids(rt_ctx* ctx, const float* x, int64_t n, int32_t* ids) {
   if (n == 0) return RT_OK;
   RT_CHECK_PTR(ctx, x);
   RT_CHECK_PTR(ctx, ids);
+  if ((const void*)x != ids && rt_overlap(x, 4 * n, ids, 4 * n)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_token_ids: ids overlaps x");
   RtOnDevice here(ctx);
   rt_launch(ctx, token_ids_kernel, rt_grid_for(ctx, n, kThreads), kThreads, 0, x, n, ids);
   RT_LAUNCHED(ctx);
@@ -586,6 +587,8 @@ rt_status rt_embedding(rt_ctx* ctx, const float* table, int64_t rows, int64_t co
   if (rows > 0) RT_CHECK_PTR(ctx, table);
   RT_CHECK_PTR(ctx, ids);
   RT_CHECK_PTR(ctx, out);
+  if (rt_overlap(out, 4 * n * cols, table, 4 * rows * cols) || rt_overlap(out, 4 * n * cols, ids, 4 * n))
+    RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_embedding: out overlaps what is read");
   RtOnDevice here(ctx);
   const bool vec = cols % 4 == 0 && rt_aligned16(table) && rt_aligned16(out);
   const int64_t pieces = vec ? cols / 4 : cols;
@@ -607,6 +610,8 @@ rt_status rt_embedding_backward(rt_ctx* ctx, const float* g, const int32_t* ids,
   if (n == 0) return accumulate ? RT_OK : rt_fill(ctx, dtable, 0.f, rows * cols);
   RT_CHECK_PTR(ctx, g);
   RT_CHECK_PTR(ctx, ids);
+  if (rt_overlap(dtable, 4 * rows * cols, g, 4 * n * cols) || rt_overlap(dtable, 4 * rows * cols, ids, 4 * n))
+    RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_embedding_backward: dtable overlaps what is read");
   RtOnDevice here(ctx);
   int bits = 1;  // of the largest key, which is `rows`
   while (bits < 32 && (uint64_t)rows >> bits) ++bits;

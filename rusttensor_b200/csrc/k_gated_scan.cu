@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(kThreads) scan_columns_kernel(const ScanArgs s
     float fs[kAhead], vs[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      fs[k] = t + k < s.steps ? __ldg(f + k * step) : 0.f;
-      vs[k] = t + k < s.steps ? __ldg(v + k * step) : 0.f;
+      fs[k] = t + k < s.steps ? f[k * step] : 0.f;  // h may be in the same place: no read-only loads
+      vs[k] = t + k < s.steps ? v[k * step] : 0.f;
     }
     f += kAhead * step;
     v += kAhead * step;
@@ -485,6 +485,20 @@ rt_status check_sizes(rt_ctx* ctx, const char* who, int64_t steps, int64_t batch
   return RT_OK;
 }
 
+// `rows` rows of `cols` values, ld apart.
+struct Rows {
+  const float* p;
+  int64_t rows, cols, ld;
+};
+// Whether they share a value: not if they are different columns of one matrix.
+bool meet(const Rows& a, const Rows& b) {
+  if (!a.p || !b.p || !rt_overlap(a.p, 4 * ((a.rows - 1) * a.ld + a.cols), b.p, 4 * ((b.rows - 1) * b.ld + b.cols))) return false;
+  const int64_t bytes = (int64_t)((intptr_t)b.p - (intptr_t)a.p);
+  if (a.ld != b.ld || bytes % 4 != 0) return true;
+  const int64_t d = (bytes / 4 % a.ld + a.ld) % a.ld;
+  return d < a.cols || a.ld - d < b.cols;
+}
+
 }  // namespace
 
 extern "C" {
@@ -498,6 +512,11 @@ rt_status rt_gated_scan(rt_ctx* ctx, const float* f, const float* v, int64_t ld,
   RT_CHECK_PTR(ctx, v);
   RT_CHECK_PTR(ctx, h);
   if (h == h0 && steps > 1) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_gated_scan: h may be h0 for a single timestep only");
+  const Rows states{h, steps * batch, hidden, hidden};
+  const bool in_place = steps == 1 && ld == hidden;
+  if ((!(in_place && h == f) && meet(states, {f, steps * batch, hidden, ld})) || (!(in_place && h == v) && meet(states, {v, steps * batch, hidden, ld})) ||
+      (h != h0 && meet(states, {h0, batch, hidden, hidden})))
+    RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_gated_scan: h overlaps what is read");
   RtOnDevice here(ctx);
   ScanArgs s{};
   s.f = f;
@@ -529,6 +548,14 @@ rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, in
   RT_CHECK_PTR(ctx, dh);
   RT_CHECK_PTR(ctx, df);
   RT_CHECK_PTR(ctx, dv);
+  const int64_t all = steps * batch;
+  const Rows read[] = {{f, all, hidden, ld}, {v, all, hidden, ld}, {h, all, hidden, hidden}, {dh, all, hidden, hidden}, {h0, batch, hidden, hidden}};
+  const Rows written[] = {{df, all, hidden, ldd}, {dv, all, hidden, ldd}, {dh0, batch, hidden, hidden}};
+  for (const Rows& w : written)
+    for (const Rows& r : read)
+      if (meet(w, r)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_gated_scan_backward: a result overlaps what is read");
+  if (meet(written[0], written[1]) || meet(written[0], written[2]) || meet(written[1], written[2]))
+    RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_gated_scan_backward: results overlap");
   RtOnDevice here(ctx);
   ScanArgs s{};
   s.f = f;

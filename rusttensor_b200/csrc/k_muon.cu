@@ -113,22 +113,22 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     p.sums[blockIdx.x] = sum;
   }
 }
-// 1 / (norm + epsilon), in every thread of a warp.
-__device__ __forceinline__ float one_over_norm(const double* __restrict__ sums) {
+// 1 / (norm + epsilon), in every thread of a warp.  In 64 bits: of the largest matrices it has no room among the normal numbers of 32.
+__device__ __forceinline__ double one_over_norm(const double* __restrict__ sums) {
   double sum = 0.0;
 #pragma unroll
   for (int b = 0; b < kNormBlocks; b += 32) sum += __ldg(sums + b + (threadIdx.x & 31));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return (float)(1.0 / (sqrt(sum) + kEpsilon));
+  return 1.0 / (sqrt(sum) + kEpsilon);
 }
 // X: the update divided by its norm, its shorter side first.
 __global__ void __launch_bounds__(kThreads) normalise_kernel(const Update u, int64_t rows, int64_t cols, const double* __restrict__ sums, float* __restrict__ x) {
   RT_PDL_ENTRY();
-  const float by = one_over_norm(sums);
+  const double by = one_over_norm(sums);
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * kThreads) {
     const int64_t r = i / cols, c = i - r * cols;
-    x[rows > cols ? c * rows + r : i] = update_at(u, i) * by;
+    x[rows > cols ? c * rows + r : i] = (float)(update_at(u, i) * by);
   }
 }
 // s = a I + b g + c s
@@ -700,7 +700,8 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
           }
         }
       }
-      // copies that nobody has waited for must have landed before the CTA may leave
+      // what the MMA warp tells of the last stages has arrived before the CTA may leave, and copies that nobody has waited for have landed
+      for (int i = it > kStages ? it - kStages : 0; ok && i < it; ++i) ok = parts::wait(empty(i % kStages), (i / kStages) & 1, p.status, 99, abort_flag);
       if (!ok && rank == 0)
         for (int i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait(full(i % kStages), (i / kStages) & 1, p.status, 92);
     }
@@ -802,7 +803,7 @@ struct Parts {
 __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__ Parts p) {
   RT_PDL_ENTRY();
   __shared__ float tile[64][65];
-  __shared__ float by;
+  __shared__ double by;
   for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < p.tickets_end; i += gridDim.x * kThreads) p.tickets[i] = 0;
   int q = 0;
   while (blockIdx.x >= p.first[q + 1]) ++q;
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   const unsigned local = blockIdx.x - p.first[q], tiles_c = (unsigned)((cols + 63) / 64);
   const int64_t r0 = (int64_t)(local / tiles_c) * 64, c0 = (int64_t)(local % tiles_c) * 64;
   if (threadIdx.x < 32) {
-    const float f = one_over_norm(p.sums[q]);
+    const double f = one_over_norm(p.sums[q]);
     if (threadIdx.x == 0) by = f;
   }
   const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
@@ -825,7 +826,7 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   const bool tall = rows > cols;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const float w = v[k] * by;
+    const float w = (float)(v[k] * by);
     if (tall) tile[lane][row + 4 * k] = w;
     else tile[row + 4 * k][lane] = w;
   }
@@ -882,12 +883,15 @@ Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
     const int units = width == 64 ? ctx->sm_count : ctx->sm_count / 2;
     for (int phase = 0; phase < 3; ++phase) {
       double least_here = 1e300;
-      for (int most = 64; most >= 1; most /= 2) {  // K-blocks of a tile at most, where that needs it split
+      int deepest = 1;
+      for (int q = 0; q < count; ++q)
+        while (deepest < ((phase == kGram ? items[q].n : items[q].m) + kBlockK - 1) / kBlockK) deepest *= 2;
+      for (int most = deepest; most >= 1; most /= 2) {  // K-blocks of a tile at most, where that needs it split
         int splits[kGroup];
         double work = 0, longest = 0;
         for (int q = 0; q < count; ++q) {
           const int blocks = ((phase == kGram ? items[q].n : items[q].m) + kBlockK - 1) / kBlockK;
-          splits[q] = most == 64 ? 1 : (blocks + most - 1) / most;
+          splits[q] = (blocks + most - 1) / most;
           const double one = block * ((blocks + splits[q] - 1) / splits[q]) + rest + (splits[q] > 1 ? (4600 + 400 * splits[q]) * (width / 64) : 0);
           work += one * (double)tiles_of(phase, width, items[q].m, items[q].n) * splits[q];
           longest = std::max(longest, one);
@@ -1067,23 +1071,15 @@ rt_status check_sizes(rt_ctx* ctx, const char* who, int count, const int64_t* ro
 }
 struct Block {
   uintptr_t begin, end;
-  int matrix;    // that it belongs to
   bool written;
 };
-Block block_of(const float* p, int64_t n, int matrix, bool written) { return {(uintptr_t)p, (uintptr_t)(p + n), matrix, written}; }
-// Whether nothing that is written overlaps anything else, `in_place` aside: what is read for a result that takes its very place.
-bool apart(std::vector<Block> blocks, bool in_place) {
+Block block_of(const float* p, int64_t n, bool written) { return {(uintptr_t)p, (uintptr_t)(p + n), written}; }
+// Whether nothing that is written overlaps anything else.
+bool apart(std::vector<Block> blocks) {
   std::sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.begin < b.begin; });
   uintptr_t end = 0, written = 0;  // of all blocks so far, of those that are written
   for (size_t i = 0; i < blocks.size(); ++i) {
     const Block& b = blocks[i];
-    if (in_place && i > 0) {
-      const Block& a = blocks[i - 1];
-      if (a.begin == b.begin && a.end == b.end && a.matrix == b.matrix && a.written != b.written) {
-        written = std::max(written, b.end);
-        continue;
-      }
-    }
     if (b.begin < (b.written ? end : written)) return false;
     end = std::max(end, b.end);
     if (b.written) written = std::max(written, b.end);
@@ -1108,8 +1104,8 @@ rt_status rt_orthogonalize_list(rt_ctx* ctx, int count, const float* const* xs, 
       if (rows[i] == 0 || cols[i] == 0) continue;
       RT_CHECK_PTR(ctx, xs[i]);
       RT_CHECK_PTR(ctx, outs[i]);
-      blocks.push_back(block_of(xs[i], rows[i] * cols[i], i, false));
-      blocks.push_back(block_of(outs[i], rows[i] * cols[i], i, true));
+      if (xs[i] != outs[i]) blocks.push_back(block_of(xs[i], rows[i] * cols[i], false));  // in place: nobody else's
+      blocks.push_back(block_of(outs[i], rows[i] * cols[i], true));
       Matrix q{};
       q.u.x = xs[i];
       q.rows = rows[i];
@@ -1117,7 +1113,7 @@ rt_status rt_orthogonalize_list(rt_ctx* ctx, int count, const float* const* xs, 
       q.out = outs[i];
       list.push_back(q);
     }
-    if (!apart(blocks, true)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_orthogonalize_list: a result overlaps another or another's matrix");
+    if (!apart(blocks)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_orthogonalize_list: a result overlaps another or another's matrix");
     RtOnDevice here(ctx);
     if ((st = orthogonalize_all(ctx, list, steps)) != RT_OK) return st;
   } catch (const std::bad_alloc&) {
@@ -1142,9 +1138,9 @@ rt_status rt_muon_step_multi(rt_ctx* ctx, int n_tensors, float* const* params, c
       RT_CHECK_PTR(ctx, params[i]);
       RT_CHECK_PTR(ctx, grads[i]);
       RT_CHECK_PTR(ctx, momenta[i]);
-      blocks.push_back(block_of(params[i], rows[i] * cols[i], i, true));
-      blocks.push_back(block_of(grads[i], rows[i] * cols[i], i, false));
-      blocks.push_back(block_of(momenta[i], rows[i] * cols[i], i, true));
+      blocks.push_back(block_of(params[i], rows[i] * cols[i], true));
+      blocks.push_back(block_of(grads[i], rows[i] * cols[i], false));
+      blocks.push_back(block_of(momenta[i], rows[i] * cols[i], true));
       Matrix q{};
       q.u = {nullptr, grads[i], momenta[i], momentum, grad_scale, nesterov};
       q.rows = rows[i];
@@ -1155,7 +1151,7 @@ rt_status rt_muon_step_multi(rt_ctx* ctx, int n_tensors, float* const* params, c
       q.step = (float)(lr * std::sqrt(std::max(1.0, (double)cols[i] / (double)rows[i])));
       list.push_back(q);
     }
-    if (!apart(blocks, false)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_muon_step_multi: a parameter or momentum overlaps another or a gradient");
+    if (!apart(blocks)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_muon_step_multi: a parameter or momentum overlaps another or a gradient");
     RtOnDevice here(ctx);
     if ((st = orthogonalize_all(ctx, list, steps)) != RT_OK) return st;
   } catch (const std::bad_alloc&) {

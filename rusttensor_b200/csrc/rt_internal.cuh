@@ -205,6 +205,10 @@ struct RtOnDevice {
   RtOnDevice& operator=(const RtOnDevice&) = delete;
 };
 
+static inline bool rt_overlap(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
+  return (uintptr_t)a < (uintptr_t)b + bytes_b && (uintptr_t)b < (uintptr_t)a + bytes_a;
+}
+
 static inline int rt_grid_for(rt_ctx* ctx, int64_t work_items, int per_block, int max_waves = 8) {
   int64_t blocks = (work_items + per_block - 1) / per_block;
   int64_t cap = (int64_t)ctx->sm_count * max_waves;

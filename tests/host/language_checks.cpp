@@ -36,6 +36,10 @@ int main() {
   EXPECT(REFUSED(rt_token_ids(&ctx, x, -1, ids), "negative"));
   EXPECT(REFUSED(rt_token_ids(&ctx, x, 1, nullptr), "ids"));
   EXPECT(rt_token_ids(&ctx, nullptr, 0, nullptr) == RT_OK);
+  EXPECT(REFUSED(rt_embedding(&ctx, x, 4, 4, ids, 2, 1.f, x + 15), "overlaps"));
+  EXPECT(REFUSED(rt_embedding(&ctx, x, 4, 4, reinterpret_cast<int32_t*>(x + 20), 2, 1.f, x + 16), "overlaps"));
+  EXPECT(REFUSED(rt_embedding_backward(&ctx, x, ids, 4, 4, 4, 1.f, x + 15, 1), "overlaps"));
+  EXPECT(REFUSED(rt_token_ids(&ctx, x, 4, reinterpret_cast<int32_t*>(x + 1)), "overlaps"));
   // gated scan
   EXPECT(REFUSED(rt_gated_scan(&ctx, x, x, 2, nullptr, -1, 1, 2, x), "negative"));
   EXPECT(REFUSED(rt_gated_scan(&ctx, x, x, 1, nullptr, 1, 1, 2, x), "apart"));
@@ -54,6 +58,18 @@ int main() {
   EXPECT(REFUSED(rt_gated_scan_backward(&ctx, x, x, 2, nullptr, x, x, 1, 1, 2, nullptr, x, 2, nullptr), "df"));
   EXPECT(REFUSED(rt_gated_scan_backward(&ctx, x, x, 2, nullptr, x, x, 1, 1, 2, x, nullptr, 2, nullptr), "dv"));
   EXPECT(rt_gated_scan_backward(&ctx, x, x, 2, nullptr, x, x, 0, 1, 2, x, x, 2, nullptr) == RT_OK);
+  // 4 rows of 2 columns: h onto f, onto v, onto another part of h0; a gradient onto each thing that is read and onto each other result
+  float z[64] = {};
+  EXPECT(REFUSED(rt_gated_scan(&ctx, x, z, 4, nullptr, 4, 1, 2, x + 12), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan(&ctx, z, x + 2, 4, nullptr, 4, 1, 2, x), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan(&ctx, z, z, 4, x + 6, 4, 1, 2, x), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan(&ctx, z, z, 4, x + 1, 1, 1, 2, x), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan_backward(&ctx, x, z + 2, 4, nullptr, z + 20, z + 30, 4, 1, 2, x + 1, x + 17, 4, nullptr), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan_backward(&ctx, z, z + 2, 4, nullptr, z + 20, x + 20, 4, 1, 2, x, x + 18, 4, nullptr), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan_backward(&ctx, z, z + 2, 4, x + 40, z + 20, z + 30, 4, 1, 2, x, x + 2, 4, x + 41), "overlaps"));
+  EXPECT(REFUSED(rt_gated_scan_backward(&ctx, z, z + 2, 4, nullptr, z + 20, z + 30, 4, 1, 2, x, x + 1, 4, nullptr), "results overlap"));
+  EXPECT(REFUSED(rt_gated_scan_backward(&ctx, z, z + 2, 4, nullptr, z + 20, z + 30, 4, 1, 2, x, x + 3, 4, nullptr), "results overlap"));
+  EXPECT(REFUSED(rt_gated_scan_backward(&ctx, z, z + 2, 4, nullptr, z + 20, z + 30, 4, 1, 2, x, x + 2, 4, x + 10), "results overlap"));
   // Muon
   float *p[2] = {x, x + 32}, *m[2] = {x + 16, x + 48}, *none[2] = {x, nullptr};
   float y[32] = {};
@@ -80,6 +96,11 @@ int main() {
   float* onto[2] = {y + 8, x};  // a result within the other's matrix
   EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, g, rows, cols, 5, onto), "overlap"));
   EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, g, rows, cols, 5, none), "outs"));
+  const float* same[2] = {y, y};  // one of the results in the place that the other is read from, in either order
+  float *in_place[2] = {y, x}, *in_place_too[2] = {x, y};
+  const int64_t square[2] = {4, 4};
+  EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, same, square, square, 5, in_place), "overlap"));
+  EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 2, same, square, square, 5, in_place_too), "overlap"));
   EXPECT(REFUSED(rt_orthogonalize_list(&ctx, 1, g, nullptr, cols, 5, p), "rows"));
   EXPECT(ctx.launches == 0);
   return failures ? 1 : 0;

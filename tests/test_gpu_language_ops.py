@@ -321,7 +321,7 @@ def test_orthogonalize_by_either_path(capi, contraction_path, steps):
         as_near_as_fp32(out.numpy(), ref.orthogonalize(x, steps), ref.orthogonalize(x, steps, np.float32))
 
 
-@pytest.mark.parametrize("value", [0.0, 1e-30, 1e30, np.nan, np.inf])
+@pytest.mark.parametrize("value", [0.0, 1e-30, 1e30, 5e37, np.nan, np.inf])
 def test_orthogonalize_of_special_matrices(capi, value):
     r = rng(32)
     for shape in ((40, 30), (150, 200)):
@@ -371,6 +371,81 @@ def test_muon_step(capi, nesterov):
         allowed = 3 * np.linalg.norm(plain - want) + 4 * ref.U * (np.linalg.norm(host[0][k]) + 2 * step * np.sqrt(min(s)))
         assert np.linalg.norm(got - want) <= allowed, s
     assert all(np.array_equal(a.numpy(), b) for a, b in zip(g, host[1]))
+
+
+@pytest.mark.parametrize("steps", [0, 5])
+def test_muon_step_by_either_path(capi, contraction_path, steps):
+    r = rng(37)
+    lr, mu, wd, scale = 0.05, 0.9, 0.02, 0.5
+    for s in ((1, 1), (40, 90), (333, 140)):
+        p0, g0, m0 = (matrix(r, s) for _ in range(3))
+        p, g, m = (capi.to_device(x) for x in (p0, g0, m0))
+        capi.call("muon_step_multi", 1, pointers([p]), pointers([g]), pointers([m]), capi.i64([s[0]]), capi.i64([s[1]]), f32(lr), f32(mu), 1, f32(wd), steps, f32(scale))
+        want, want_m = ref.muon(p0, g0, m0, lr, mu, 1, wd, steps, scale)
+        plain, _ = ref.muon(p0, g0, m0, lr, mu, 1, wd, steps, scale, np.float32)
+        assert within(m.numpy(), want_m, 2 * ref.U * (np.abs(mu * m0) + np.abs(scale * g0)))
+        step = lr * max(1.0, s[1] / s[0]) ** 0.5
+        # the update is off by no more than one step and its growth (as_near_as_fp32); keeping, subtracting: rounded three times
+        allowed = 3 * np.linalg.norm(plain - want) + step * 301 * ref.U + 4 * ref.U * (np.linalg.norm(p0) + 2 * step * np.sqrt(min(s)))
+        assert np.linalg.norm(p.numpy() - want) <= allowed, s
+
+
+def test_two_contexts_at_once(capi):
+    """Cooperative launches, small and large, on two streams: the same bits as one after the other."""
+    r = rng(38)
+    lists = [[(300, 200), (90, 40)], [(1501, 1603)], [(1290, 1803)] * 6]
+    other = rusttensor_b200.CApi()
+    try:
+        host = [[matrix(r, s) for s in shapes] for shapes in lists]
+        results = []
+        for apis in ((capi, capi), (capi, other)):
+            work = [(api, xs, [api.to_device(x) for x in xs], [api.empty(x.shape) for x in xs]) for api in apis for xs in host]
+            for api in apis:
+                api.sync()
+            for _ in range(3):
+                for k in range(len(lists)):
+                    for api, xs, d, o in (work[k], work[len(lists) - 1 - k + len(lists)]):
+                        api.call("orthogonalize_list", len(xs), pointers(d), api.i64([x.shape[0] for x in xs]), api.i64([x.shape[1] for x in xs]), 5, pointers(o))
+            results.append([[a.numpy() for a in o] for _, _, _, o in work])
+            for api in apis:
+                code = C.c_int(0)
+                api.call("device_status", C.byref(code))
+        for one, two in zip(*results):
+            assert all(np.array_equal(a, b) for a, b in zip(one, two))
+    finally:
+        other.close()
+
+
+def test_large_matrices_captured_and_replayed(capi):
+    """Two graphs of the same call, an eager call between their launches."""
+    r = rng(39)
+    shapes = [(1501, 1603), (65, 700)]
+    d, o = [capi.empty(s) for s in shapes], [capi.empty(s) for s in shapes]
+    args = (len(shapes), pointers(d), capi.i64([s[0] for s in shapes]), capi.i64([s[1] for s in shapes]), 5, pointers(o))
+    inputs = [[matrix(r, s) for s in shapes] for _ in range(2)]
+
+    def fill(k):
+        for x, dx in zip(inputs[k], d):
+            capi.check(capi.lib.rt_memcpy_h2d(capi.ctx, dx.ptr, x.ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes)))
+
+    want, graphs = [], []
+    for k in range(2):
+        fill(k)
+        capi.call("orthogonalize_list", *args)
+        want.append([x.numpy() for x in o])
+    for _ in range(2):
+        capi.call("graph_begin")
+        capi.call("orthogonalize_list", *args)
+        graphs.append(C.c_void_p())
+        capi.call("graph_end", C.byref(graphs[-1]))
+    for graph, k in ((0, 0), (1, 1), (0, 1), (1, 0)):
+        fill(1 - k)
+        capi.call("orthogonalize_list", *args)
+        fill(k)
+        capi.call("graph_launch", graphs[graph])
+        assert all(np.array_equal(a.numpy(), b) for a, b in zip(o, want[k]))
+    for g in graphs:
+        capi.call("graph_destroy", g)
 
 
 # ---- in graphs, through the engine, together ------------------------------------------------------------------------------------------------
