@@ -869,9 +869,15 @@ int64_t tiles_of(int phase, int width, int64_t m, int64_t n) {
   const int64_t all = rows * (rows + 1);
   return (rows - 1) * height + width >= m ? all - 1 : all;  // the last one has no columns
 }
-// In cycles, as measured: a K-block, what a tile takes besides, what sharing a reduction takes.  Microseconds with 64, 128 and 256 columns: 512 x 512 158,
-// 204 and 339; 1024 x 1024 218, 288 and 447; 2000 x 2600 1093, 786 and 911; with 128 and 256 columns
-// 4096 x 4096 4480 and 3585.
+// What a tile takes in cycles: for a K-block, besides, if its reduction is shared, and for each CTA that shares it.  A product takes as many rounds as its
+// work items need at one per CTA or pair, of the time that they take on average.  Fitted to 55 measurements, from 64 x 64 to 4096 x 4096 and 300 x 20000 and
+// lists of up to 12, with each of the widths and two ways to share reductions: within 5 to 7 % (root of the mean square).  Microseconds with 64,
+// 128 and 256 columns: 512 x 512 158, 206 and 340; 1400 x 1400 378, 378 and 553; 2048 x 2048 929, 638 and 756; 3000 x 3500 3227, 2477 and
+// 2297; five matrices up to 2048 wide 501, 369 and 630.
+struct Cost {
+  double block, rest, shared, share;
+};
+constexpr Cost kCosts[3] = {{1140, 7600, 3600, 500}, {1400, 12600, 7000, 950}, {2230, 23900, 12200, 3900}};
 Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
   Plan best{};
   double least = 1e300;
@@ -879,7 +885,7 @@ Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
     Plan p{};
     p.width = width;
     double sum = 0;
-    const double block = width == 256 ? 1550 : (width == 128 ? 1000 : 1050), rest = width == 256 ? 22000 : (width == 128 ? 11000 : 4500);
+    const Cost& cost = kCosts[width / 128];
     const int units = width == 64 ? ctx->sm_count : ctx->sm_count / 2;
     for (int phase = 0; phase < 3; ++phase) {
       double least_here = 1e300;
@@ -888,15 +894,17 @@ Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
         while (deepest < ((phase == kGram ? items[q].n : items[q].m) + kBlockK - 1) / kBlockK) deepest *= 2;
       for (int most = deepest; most >= 1; most /= 2) {  // K-blocks of a tile at most, where that needs it split
         int splits[kGroup];
-        double work = 0, longest = 0;
+        double work = 0, tiles = 0, longest = 0;
         for (int q = 0; q < count; ++q) {
           const int blocks = ((phase == kGram ? items[q].n : items[q].m) + kBlockK - 1) / kBlockK;
           splits[q] = (blocks + most - 1) / most;
-          const double one = block * ((blocks + splits[q] - 1) / splits[q]) + rest + (splits[q] > 1 ? (4600 + 400 * splits[q]) * (width / 64) : 0);
-          work += one * (double)tiles_of(phase, width, items[q].m, items[q].n) * splits[q];
+          const double one = cost.block * ((blocks + splits[q] - 1) / splits[q]) + cost.rest + (splits[q] > 1 ? cost.shared + cost.share * splits[q] : 0);
+          const double all = (double)tiles_of(phase, width, items[q].m, items[q].n) * splits[q];
+          work += one * all;
+          tiles += all;
           longest = std::max(longest, one);
         }
-        const double time = std::max(longest, work / units) + 0.5 * longest;  // the last tiles do not all end at once
+        const double time = std::max(longest, std::ceil(tiles / units) * work / tiles);
         if (time < least_here) {
           least_here = time;
           std::copy(splits, splits + count, p.splits[phase]);
