@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) scan_columns_backward_kernel(const S
 // units of C / V lanes one after the other in time; then come the warps of a block and the blocks of a cluster (backward: against time).
 constexpr int kMaxWarps = 8, kMaxCluster = 8;
 struct Exchange {
-  float2 of_warp[kMaxWarps][32];                // A and B
+  float2 of_warp[2][kMaxWarps][32];             // A and B, turn by turn: a warp may be one ahead of another that still reads
   float2 of_block[2][kMaxCluster][32];          // of the cluster's blocks, turn by turn
   uint64_t arrived[2];                          // barriers that count the bytes of those
 };
@@ -205,7 +205,7 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
   }
   if (unit == kUnits - 1) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) x.of_warp[warp][lane % kLanes * V + j] = make_float2(pa[j], pb[j]);
+    for (int j = 0; j < V; ++j) x.of_warp[turn & 1][warp][lane % kLanes * V + j] = make_float2(pa[j], pb[j]);
   }
   __syncthreads();
   // from here on the lane is the column (lanes beyond C: nobody asks for theirs)
@@ -215,7 +215,7 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
       wa = ba;
       wb = bb;
     }
-    const float2 q = x.of_warp[w][lane];
+    const float2 q = x.of_warp[turn & 1][w][lane];
     bb = q.x * bb + q.y;
     ba = q.x * ba;
   }
@@ -232,7 +232,6 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
     }
   } else {
     state = ba * state + bb;
-    __syncthreads();  // of_warp is written again
   }
   before = wa * before + wb;
 #pragma unroll
