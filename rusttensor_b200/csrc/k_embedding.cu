@@ -327,13 +327,21 @@ __device__ __forceinline__ void write_row(const Runs& r, uint32_t row, int64_t c
   if (ACCUMULATE) P::add(sum, old);
   *(reinterpret_cast<typename P::T*>(r.dtable + (int64_t)row * r.cols) + c) = sum;
 }
-// The first of the sorted pairs whose key is not below `key`.
+// The first of the sorted pairs whose key is not below `key`; seven looks at a time, which do not wait for one another.
 __device__ __forceinline__ uint32_t first_of(const uint2* __restrict__ pairs, uint32_t n, uint32_t key) {
   uint32_t lo = 0, hi = n;
   while (lo < hi) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (__ldg(&pairs[mid].x) < key) lo = mid + 1;
-    else hi = mid;
+    const uint32_t step = (hi - lo + 7) / 8;
+    uint32_t seen[7], below = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 7; ++j) {
+      const uint32_t at = lo + step * (j + 1) - 1;
+      seen[j] = at < hi ? __ldg(&pairs[at].x) : ~0u;  // no key is that large
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 7; ++j) below += seen[j] < key;
+    lo += step * below;
+    if (below < 7) hi = min(hi, lo + step - 1);
   }
   return lo;
 }
@@ -372,21 +380,14 @@ __global__ void __launch_bounds__(kSumThreads) run_sums_kernel(const Runs r) {
   const uint32_t terms = __popc(__ballot_sync(0xffffffffu, mine.x < r.rows));  // padding comes last
   if (terms == 0) return;
   const uint32_t first = __shfl_sync(0xffffffffu, mine.x, 0), last = __shfl_sync(0xffffffffu, mine.x, count - 1);
-  bool head = begin > 0 && __ldg(&r.pairs[begin - 1].x) == first;  // the run began in a tile before
-  const bool goes_on = terms == kRun && begin + kRun < r.n && __ldg(&r.pairs[begin + kRun].x) == last;
+  const uint32_t key_before = begin > 0 ? __ldg(&r.pairs[begin - 1].x) : ~0u, key_behind = begin + kRun < r.n ? __ldg(&r.pairs[begin + kRun].x) : ~0u;
   const uint32_t behind = __shfl_down_sync(0xffffffffu, mine.x, 1);
   const uint32_t ends = __ballot_sync(0xffffffffu, lane + 1 == terms || mine.x != behind);  // of runs
-  if (c == 0 && goes_on && !(head && first == last)) {
-    const uint32_t far = begin + kRun * (kShort + 1), longer = far < r.n && __ldg(&r.pairs[far].x) == last;
-    const uint32_t k = atomicAdd(r.crossing + longer, 1u);
-    r.crossing[2 + (longer ? r.tiles - 1 - k : k)] = t;
-  }
   const bool in = c < pieces;
   T* parts = reinterpret_cast<T*>(r.parts + (int64_t)t * 2 * r.cols) + c;
   const T *g = reinterpret_cast<const T*>(r.g) + c, *table = reinterpret_cast<const T*>(r.dtable) + c;
-  T sum = P::zero();
-  for (uint32_t i = 0; i < terms; i += 8) {
-    T v[8], old[8] = {};
+  T sum = P::zero(), v[8], old[8] = {};
+  auto load = [&](uint32_t i) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t place = __shfl_sync(0xffffffffu, mine.y, i + k);
@@ -399,6 +400,13 @@ __global__ void __launch_bounds__(kSumThreads) run_sums_kernel(const Runs r) {
         old[k] = in && i + k < terms && ends >> (i + k) & 1 ? table[(int64_t)row * pieces] : P::zero();
       }
     }
+  };
+  load(0);  // before anybody waits for the neighbours' keys
+  const bool began = key_before == first;                    // in a tile before
+  const bool goes_on = terms == kRun && key_behind == last;  // behind this one
+  bool head = began;
+  for (uint32_t i = 0; i < terms; i += 8) {
+    if (i > 0) load(i);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       P::add(sum, v[k]);
@@ -413,6 +421,11 @@ __global__ void __launch_bounds__(kSumThreads) run_sums_kernel(const Runs r) {
         sum = P::zero();
       }
     }
+  }
+  if (c == 0 && goes_on && !(began && first == last)) {
+    const uint32_t far = begin + kRun * (kShort + 1), longer = far < r.n && __ldg(&r.pairs[far].x) == last;
+    const uint32_t k = atomicAdd(r.crossing + longer, 1u);
+    r.crossing[2 + (longer ? r.tiles - 1 - k : k)] = t;
   }
 }
 // The parts of the runs that go over the ends of tiles, in the order of the tiles.  Short runs: a warp has 32 pieces of the columns of one.  Long
@@ -439,19 +452,29 @@ __global__ void __launch_bounds__(kJoinThreads) join_runs_kernel(const Runs r) {
   __shared__ T of_warp[kJoinThreads / 32][32];
   const int64_t pieces = VEC ? r.cols / 4 : r.cols;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kJoinThreads / 32;
+  // from the last block on: where there is little work, the first ones have the long runs
+  const int64_t w0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * warps + warp;
+  const uint32_t t0 = w0 / r.slabs < r.tiles ? __ldg(r.crossing + 2 + w0 / r.slabs) : 0;  // of use if there are so many
   const int64_t shorts = (int64_t)__ldg(r.crossing) * r.slabs, longs = (int64_t)__ldg(r.crossing + 1) * r.slabs;
   const T* table = reinterpret_cast<const T*>(r.dtable);
-  // from the last block on: where there is little work, the first ones have the long runs
-  for (int64_t w = (int64_t)(gridDim.x - 1 - blockIdx.x) * warps + warp; w < shorts; w += (int64_t)gridDim.x * warps) {
-    const uint32_t t = __ldg(r.crossing + 2 + w / r.slabs), q = t + 1 + lane;
+  for (int64_t w = w0; w < shorts; w += (int64_t)gridDim.x * warps) {
+    const uint32_t t = w == w0 ? t0 : __ldg(r.crossing + 2 + w / r.slabs), q = t + 1 + lane;
+    const int64_t c = w % r.slabs * 32 + lane;
+    const bool in = c < pieces;
+    const T* parts = reinterpret_cast<const T*>(r.parts) + (in ? c : 0);
+    // the parts of the first tiles are on their way while it is found out how many there are
+    T sum = parts[(int64_t)t * 2 * pieces + pieces], v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) v[k] = t + 1 + k < r.tiles ? parts[(int64_t)(t + 1 + k) * 2 * pieces] : P::zero();
     const uint32_t run = __ldg(&r.pairs[t * kRun + kRun - 1].x);
     // how many tiles behind this one begin with the run
     const uint32_t count = __popc(__ballot_sync(0xffffffffu, q < r.tiles && __ldg(&r.pairs[q * kRun].x) == run));
-    const int64_t c = w % r.slabs * 32 + lane;
-    if (c >= pieces) continue;
+    if (!in) continue;
     const T old = ACCUMULATE ? table[(int64_t)run * pieces + c] : P::zero();
-    const T* parts = reinterpret_cast<const T*>(r.parts) + c;
-    write_row<VEC, ACCUMULATE>(r, run, c, add_parts<VEC>(parts, pieces, t + 1, t + 1 + count, parts[(int64_t)t * 2 * pieces + pieces]), old);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (k < count) P::add(sum, v[k]);
+    write_row<VEC, ACCUMULATE>(r, run, c, count > 4 ? add_parts<VEC>(parts, pieces, t + 5, t + 1 + count, sum) : sum, old);
   }
   for (int64_t w = blockIdx.x; w < longs; w += gridDim.x) {
     const uint32_t t = __ldg(r.crossing + 2 + r.tiles - 1 - w / r.slabs), run = __ldg(&r.pairs[t * kRun + kRun - 1].x);
