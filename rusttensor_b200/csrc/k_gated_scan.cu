@@ -14,9 +14,12 @@
 //
 // Bound by memory, 12 bytes an element forward and 24 backward, and near that by the instructions (about 40 and 60 an element; 88 backward
 // with one column at a time).  Measured, in TB/s of those bytes: 128 timesteps of 64 x 512 11.7 us forward (4.3), 19.5 backward (5.2); 1000 of
-// 16 x 1000 38.3 (5.0); 65536 of 1 x 512 83.8 (4.8) and 163 (4.9); 30011 of 3 x 257 backward 156 (3.6).  A thread per column, which reads ahead
+// 16 x 1000 38.3 (5.0); 65536 of 1 x 512 85 (4.8) and 166 (4.9); 30011 of 3 x 257 backward 131 (4.2).  A thread per column, which reads ahead
 // eight timesteps, takes 24 us for the first and 9.4 ms for the third; it remains for up to eight timesteps.
 #include <cooperative_groups.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "rt_internal.cuh"
 #include "tc_common.cuh"
@@ -116,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) scan_columns_backward_kernel(const S
 // ---- stretches ------------------------------------------------------------------------------------------------------------------------
 // A block has C = 16 or 32 columns.  A thread has V of them (128-bit accesses where everything is aligned, V = 4) and S timesteps, a warp several
 // units of C / V lanes one after the other in time; then come the warps of a block and the blocks of a cluster (backward: against time).
-constexpr int kMaxWarps = 8, kMaxCluster = 8;
+constexpr int kMaxWarps = 16, kMaxCluster = 8, kAloneWarps = 8;  // of a block in a cluster; blocks; of a block by itself
 struct Exchange {
   float2 of_warp[2][kMaxWarps][32];             // A and B, turn by turn: a warp may be one ahead of another that still reads
   float2 of_block[2][kMaxCluster][32];          // of the cluster's blocks, turn by turn
@@ -239,7 +242,7 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
 }
 
 template <int C, int V, int S, bool CLUSTER>
-__global__ void __launch_bounds__(kMaxWarps * 32, CLUSTER ? 2 : 4) scan_stretches_kernel(const ScanArgs s, int blocks) {
+__global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUSTER ? 1 : 4) scan_stretches_kernel(const ScanArgs s, int blocks) {
   RT_PDL_ENTRY();
   __shared__ Exchange x;
   constexpr int kLanes = C / V;
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, CLUSTER ? 2 : 4) scan_stretche
 
 // The same against time, for e_t = a_t d_t = a_t e_{t+1} + a_t dh_t, from which d_t = dh_t + e_{t+1}.
 template <int C, int V, int S, bool CLUSTER>
-__global__ void __launch_bounds__(kMaxWarps * 32, CLUSTER ? 2 : 4) scan_stretches_backward_kernel(const ScanArgs s, int blocks) {
+__global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUSTER ? 1 : 4) scan_stretches_backward_kernel(const ScanArgs s, int blocks) {
   RT_PDL_ENTRY();
   __shared__ Exchange x;
   constexpr int kLanes = C / V;
@@ -421,24 +424,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, CLUSTER ? 2 : 4) scan_stretche
   if (s.dh0 && rank == 0 && threadIdx.x < C && col0 + lane < columns) s.dh0[col0 + lane] = state;
 }
 
-// How a sequence is cut: columns and warps of a block, blocks of a cluster.  Clusters while the columns alone do not occupy the SMs; strips of 16
-// columns (64 bytes of a row) while those of 32 leave half of the SMs without a second block.
+// How a sequence is cut: columns and warps of a block, blocks of a cluster; a block by itself has no other kind.
 struct Cut {
   int columns, warps, blocks;
   int64_t strips;
 };
-Cut cut(const rt_ctx* ctx, int64_t steps, int64_t columns, int thread_values) {
-  for (int width = 32;; width = 16) {
-    const int warp_steps = thread_values * 32 / width;
-    const int64_t strips = (columns + width - 1) / width, stretches = (steps + warp_steps - 1) / warp_steps;
-    const int warps = (int)(stretches < kMaxWarps ? stretches : kMaxWarps);
-    int blocks = 1;
-    while (blocks < kMaxCluster && strips * blocks < 2 * ctx->sm_count && blocks * warps < stretches) blocks *= 2;
-    if (width == 16 || blocks < kMaxCluster || strips * blocks > ctx->sm_count) return {width, warps, blocks, strips};
-  }
-}
+// Clusters that the SMs hold at once, with blocks of 8 warps and of 16.
+struct Fits {
+  int clusters[2][kMaxCluster + 1];
+};
 template <class Kernel>
-rt_status launch_stretches(rt_ctx* ctx, Kernel kern, const ScanArgs& s, const Cut& c) {
+rt_status launch_stretches(rt_ctx* ctx, Kernel kern, const ScanArgs& s, const Cut& c, int* fits = nullptr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = (unsigned)(c.strips * c.blocks);
   cfg.blockDim = (unsigned)c.warps * 32;
@@ -451,22 +447,75 @@ rt_status launch_stretches(rt_ctx* ctx, Kernel kern, const ScanArgs& s, const Cu
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = c.blocks > 1 ? 2 : 1;
+  if (fits) {
+    RT_CUDA(ctx, cudaOccupancyMaxActiveClusters(fits, kern, &cfg));
+    return RT_OK;
+  }
   RT_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, s, c.blocks));
   RT_LAUNCHED(ctx);
   return RT_OK;
 }
+// Asked once a device, of the kernel that needs most: how clusters lie in groups of SMs is the device's (148 SMs hold 15 of 8 blocks if a block takes
+// an SM, 26 of 5).
+rt_status fits_of(rt_ctx* ctx, Fits* fits) {
+  constexpr int kDevices = 64;  // beyond: asked every time
+  static std::atomic<int> known[kDevices][2][kMaxCluster + 1];
+  for (int k = 0; k < 2; ++k)
+    for (int blocks = 2; blocks <= kMaxCluster; ++blocks) {
+      int& n = fits->clusters[k][blocks];
+      if (ctx->device < kDevices && (n = known[ctx->device][k][blocks].load(std::memory_order_relaxed)) > 0) continue;
+      rt_status st = launch_stretches(ctx, scan_stretches_backward_kernel<32, 4, 2, true>, ScanArgs{}, Cut{32, 8 << k, blocks, 1}, &n);
+      if (st != RT_OK) return st;
+      n = std::max(n, 1);
+      if (ctx->device < kDevices) known[ctx->device][k][blocks].store(n, std::memory_order_relaxed);
+    }
+  return RT_OK;
+}
+// What takes the fewest rounds of stretches, two more (by itself: one) for a cluster's start, and as often as the clusters do not fit at once.  A
+// round takes about 2.7 us if SMs have 16 warps and 0.65 of it with 8; with strips of 16 columns, 64 bytes of a row, a little longer, and a lot
+// if rows are not aligned to sectors; without a cluster longer, too, since it waits for its loads.  30011 timesteps of 771 columns, backward:
+// five blocks of 16 warps 132 us, eight of 8 164; 65536 of 512: 32 columns and eight of 8 warps 130, 16 columns 85; 40000 of 300, backward:
+// six of 16 warps and 16 columns 91, eight of 8 115.
+rt_status cut(rt_ctx* ctx, int64_t steps, int64_t columns, int v, int s, Cut* best) {
+  Fits fits{};
+  rt_status st = fits_of(ctx, &fits);
+  if (st != RT_OK) return st;
+  double least = 1e300;
+  for (int width = 32; width >= 16; width /= 2) {
+    const int warp_steps = v * s * 32 / width;
+    const int64_t strips = (columns + width - 1) / width, stretches = (steps + warp_steps - 1) / warp_steps;
+    for (int k = 0; k < 2; ++k) {
+      const int warps = (int)std::min<int64_t>(stretches, 8 << k);
+      for (int blocks = 1; blocks <= kMaxCluster && (blocks - 1) * warps < stretches; ++blocks) {
+        if (blocks == 1 && (width == 16 || warps > kAloneWarps)) continue;
+        const int64_t fit = blocks == 1 ? 4 * (int64_t)ctx->sm_count : fits.clusters[k][blocks];
+        const double round = (blocks == 1 ? 1.3 : (width == 32 ? 1.0 : (v == 1 ? 1.4 : 1.02))) * (blocks > 1 && k == 0 && strips <= fits.clusters[1][blocks] ? 0.65 : 1.0);
+        const double time = (double)((strips + fit - 1) / fit) * (double)((stretches + blocks * warps - 1) / (blocks * warps) + (blocks > 1 ? 2 : 1)) * round;
+        if (time < least) {
+          least = time;
+          *best = {width, warps, blocks, strips};
+        }
+      }
+    }
+  }
+  return RT_OK;
+}
 template <int V, int S>
 rt_status launch_forward(rt_ctx* ctx, const ScanArgs& s) {
-  const Cut c = cut(ctx, s.steps, s.batch * s.hidden, V * S);
-  if (c.columns == 16) return launch_stretches(ctx, scan_stretches_kernel<16, V, S, true>, s, c);
-  return c.blocks > 1 ? launch_stretches(ctx, scan_stretches_kernel<32, V, S, true>, s, c) : launch_stretches(ctx, scan_stretches_kernel<32, V, S, false>, s, c);
+  Cut c{};
+  rt_status st = cut(ctx, s.steps, s.batch * s.hidden, V, S, &c);
+  if (st != RT_OK) return st;
+  if (c.blocks == 1) return launch_stretches(ctx, scan_stretches_kernel<32, V, S, false>, s, c);
+  return c.columns == 16 ? launch_stretches(ctx, scan_stretches_kernel<16, V, S, true>, s, c) : launch_stretches(ctx, scan_stretches_kernel<32, V, S, true>, s, c);
 }
 template <int V, int S>
 rt_status launch_backward(rt_ctx* ctx, const ScanArgs& s) {
-  const Cut c = cut(ctx, s.steps, s.batch * s.hidden, V * S);
-  if (c.columns == 16) return launch_stretches(ctx, scan_stretches_backward_kernel<16, V, S, true>, s, c);
-  return c.blocks > 1 ? launch_stretches(ctx, scan_stretches_backward_kernel<32, V, S, true>, s, c)
-                      : launch_stretches(ctx, scan_stretches_backward_kernel<32, V, S, false>, s, c);
+  Cut c{};
+  rt_status st = cut(ctx, s.steps, s.batch * s.hidden, V, S, &c);
+  if (st != RT_OK) return st;
+  if (c.blocks == 1) return launch_stretches(ctx, scan_stretches_backward_kernel<32, V, S, false>, s, c);
+  return c.columns == 16 ? launch_stretches(ctx, scan_stretches_backward_kernel<16, V, S, true>, s, c)
+                         : launch_stretches(ctx, scan_stretches_backward_kernel<32, V, S, true>, s, c);
 }
 // Whether four columns of every matrix can be had at once.
 bool aligned(const ScanArgs& s) {

@@ -133,7 +133,7 @@ def test_token_ids(capi):
 # ---- gated linear recurrence ---------------------------------------------------------------------------------------------------------------
 
 # (steps, batch, hidden)
-SEQUENCES = [(1, 1, 1), (1, 64, 512), (2, 3, 5), (7, 2, 33), (31, 1, 4), (128, 3, 64), (257, 2, 130), (1000, 1, 7), (1025, 5, 36), (2049, 1, 257), (33, 1, 4100), (5000, 1, 64), (9001, 2, 3)]
+SEQUENCES = [(1, 1, 1), (1, 64, 512), (2, 3, 5), (7, 2, 33), (31, 1, 4), (128, 3, 64), (257, 2, 130), (1000, 1, 7), (1025, 5, 36), (2049, 1, 257), (33, 1, 4100), (5000, 1, 64), (9001, 2, 3), (6007, 3, 257), (9000, 1, 320), (20000, 1, 40)]
 
 
 def sequence(r, steps, batch, hidden):
