@@ -113,22 +113,24 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     p.sums[blockIdx.x] = sum;
   }
 }
-// 1 / (norm + epsilon), in every thread of a warp.  In 64 bits: of the largest matrices it has no room among the normal numbers of 32.
-__device__ __forceinline__ double one_over_norm(const double* __restrict__ sums) {
+// 1 / (norm + epsilon), in every thread of a warp, as a product of two numbers: of the largest matrices it has no room among the normal numbers of
+// 32 bits.  The first one is a power of two.
+__device__ __forceinline__ float2 one_over_norm(const double* __restrict__ sums) {
   double sum = 0.0;
 #pragma unroll
   for (int b = 0; b < kNormBlocks; b += 32) sum += __ldg(sums + b + (threadIdx.x & 31));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return 1.0 / (sqrt(sum) + kEpsilon);
+  const double by = 1.0 / (sqrt(sum) + kEpsilon);
+  return by < 0x1p-100 ? make_float2(0x1p-64f, (float)(by * 0x1p64)) : make_float2(1.f, (float)by);
 }
 // X: the update divided by its norm, its shorter side first.
 __global__ void __launch_bounds__(kThreads) normalise_kernel(const Update u, int64_t rows, int64_t cols, const double* __restrict__ sums, float* __restrict__ x) {
   RT_PDL_ENTRY();
-  const double by = one_over_norm(sums);
+  const float2 by = one_over_norm(sums);
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * kThreads) {
     const int64_t r = i / cols, c = i - r * cols;
-    x[rows > cols ? c * rows + r : i] = (float)(update_at(u, i) * by);
+    x[rows > cols ? c * rows + r : i] = update_at(u, i) * by.x * by.y;
   }
 }
 // s = a I + b g + c s
@@ -803,7 +805,7 @@ struct Parts {
 __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__ Parts p) {
   RT_PDL_ENTRY();
   __shared__ float tile[64][65];
-  __shared__ double by;
+  __shared__ float2 by;
   for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < p.tickets_end; i += gridDim.x * kThreads) p.tickets[i] = 0;
   int q = 0;
   while (blockIdx.x >= p.first[q + 1]) ++q;
@@ -812,7 +814,7 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   const unsigned local = blockIdx.x - p.first[q], tiles_c = (unsigned)((cols + 63) / 64);
   const int64_t r0 = (int64_t)(local / tiles_c) * 64, c0 = (int64_t)(local % tiles_c) * 64;
   if (threadIdx.x < 32) {
-    const double f = one_over_norm(p.sums[q]);
+    const float2 f = one_over_norm(p.sums[q]);
     if (threadIdx.x == 0) by = f;
   }
   const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
@@ -826,7 +828,7 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   const bool tall = rows > cols;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const float w = (float)(v[k] * by);
+    const float w = v[k] * by.x * by.y;
     if (tall) tile[lane][row + 4 * k] = w;
     else tile[row + 4 * k][lane] = w;
   }
