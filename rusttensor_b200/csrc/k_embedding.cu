@@ -115,16 +115,23 @@ __global__ void __launch_bounds__(kThreads) digit_counts_kernel(const Pass p) {
   __syncthreads();
   p.counts[(int64_t)threadIdx.x * p.blocks + blockIdx.x] = count[threadIdx.x];
 }
-// Exclusive sums over [digit][block], one block of 1024 threads.
+// Exclusive sums over [digit][block], one block of 1024 threads, each with eight of them at a time (a million tokens: with one 56 us a pass).
 __global__ void __launch_bounds__(1024) digit_places_kernel(uint32_t* counts, int64_t n) {
   RT_PDL_ENTRY();
+  constexpr int kEach = 8;  // n is a multiple of it
   __shared__ uint32_t of_warp[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t before = 0;
-  for (int64_t first = 0; first < n; first += 1024) {
-    const int64_t i = first + threadIdx.x;
-    const uint32_t v = i < n ? counts[i] : 0u;
-    uint32_t sum = v;
+  for (int64_t first = 0; first < n; first += 1024 * kEach) {
+    const int64_t i = first + threadIdx.x * kEach;
+    uint2 v[kEach / 2];
+    uint32_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < kEach / 2; ++k) {
+      v[k] = i < n ? *reinterpret_cast<const uint2*>(counts + i + 2 * k) : make_uint2(0u, 0u);
+      mine += v[k].x + v[k].y;
+    }
+    uint32_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
@@ -138,8 +145,14 @@ __global__ void __launch_bounds__(1024) digit_places_kernel(uint32_t* counts, in
       const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += u;
     }
-    const uint32_t mine = __shfl_sync(0xffffffffu, upto - all, warp);
-    if (i < n) counts[i] = before + mine + sum - v;
+    uint32_t at = before + __shfl_sync(0xffffffffu, upto - all, warp) + sum - mine;
+    if (i < n) {
+#pragma unroll
+      for (int k = 0; k < kEach / 2; ++k) {
+        *reinterpret_cast<uint2*>(counts + i + 2 * k) = make_uint2(at, at + v[k].x);
+        at += v[k].x + v[k].y;
+      }
+    }
     before += __shfl_sync(0xffffffffu, upto, 31);
     __syncthreads();
   }
