@@ -819,10 +819,15 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
   }
   const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
   float v[16];
+  const int64_t at = (r0 + row) * cols + c0 + lane, jump = 4 * cols;
+  const int left = c0 + lane < cols ? (int)min((int64_t)64, rows - r0) - row : 0;
+  const float* from = (u.g ? (u.nesterov ? u.g : u.m) : u.x) + at;  // of the update, what there is one of (update_at)
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const int64_t r = r0 + row + 4 * k, c = c0 + lane;
-    v[k] = r < rows && c < cols ? update_at(u, r * cols + c) : 0.f;
+  for (int k = 0; k < 16; ++k, from += jump) v[k] = 4 * k < left ? *from : 0.f;
+  if (u.g && u.nesterov) {
+    const float* m = u.m + at;
+#pragma unroll
+    for (int k = 0; k < 16; ++k, m += jump) v[k] = u.scale * v[k] + (4 * k < left ? u.mu * *m : 0.f);
   }
   __syncthreads();
   const bool tall = rows > cols;
@@ -833,19 +838,17 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
     else tile[row + 4 * k][lane] = w;
   }
   __syncthreads();
-  const int64_t m = tall ? cols : rows, n = tall ? rows : cols, y0 = tall ? c0 : r0, x0 = tall ? r0 : c0, ld = p.ldx[q], plane = m * ld;
-  const int pair = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t m = tall ? cols : rows, y0 = tall ? c0 : r0, x0 = tall ? r0 : c0, ld = p.ldx[q], plane = m * ld;
+  const int pair = threadIdx.x & 31, y = threadIdx.x >> 5, high = x0 + 2 * pair < ld ? (int)min((int64_t)64, m - y0) - y : 0;  // the padding of a row: zeros
+  uint16_t* o = p.x[q] + (y0 + y) * ld + x0 + 2 * pair;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t gy = y0 + y + 8 * k, gx = x0 + 2 * pair;
-    if (gy >= m || gx >= ld) continue;  // the padding of a row: zeros
+  for (int k = 0; k < 8; ++k, o += 8 * ld) {
+    if (8 * k >= high) break;
     uint32_t hi, lo;
     split2(tile[y + 8 * k][2 * pair], tile[y + 8 * k][2 * pair + 1], hi, lo);
-    uint16_t* o = p.x[q] + gy * ld + gx;
     *reinterpret_cast<uint32_t*>(o) = hi;
     *reinterpret_cast<uint32_t*>(o + plane) = lo;
   }
-  (void)n;
 }
 
 // [2 planes][rows][cols] halves, rows ld apart, boxes of 64 columns and `height` rows of both planes, zeros outside.
