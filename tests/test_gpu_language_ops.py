@@ -537,6 +537,24 @@ def test_a_recurrent_language_model(gpu_engine, oracle_engine):
         assert np.all(np.abs(a - b) <= 1e-4 * np.maximum(np.abs(a), np.abs(b)) + 1e-4 * np.abs(b).max())
 
 
+def test_muon_with_a_parameter_listed_twice(gpu_engine, oracle_engine):
+    """It is updated twice, in order; two backward passes before a step add up; a parameter that is another's gradient is read before it changes."""
+    r = rng(53)
+    init, other = (r.standard_normal((12, 20)).astype(np.float32) for _ in range(2))
+    seen = []
+    for e in (gpu_engine, oracle_engine):
+        a, b = e.tensor(init, requires_grad=True), e.tensor(other, requires_grad=True)
+        opt = e.Muon([a, b, a], 0.05, 0.9, False, 0.01)
+        for _ in range(3):
+            for _ in range(2):
+                e.ops.sum(e.ops.mul(a, b)).backward()
+            opt.step()
+            opt.zero_grad()
+        seen.append([a.numpy(), b.numpy()])
+    for x, y in zip(*seen):
+        assert np.all(np.abs(x - y) <= 1e-4 * np.maximum(np.abs(x), np.abs(y)) + 1e-4 * np.abs(y).max())
+
+
 def test_engine_gradient_after_the_result_was_written_from_outside(gpu_engine):
     """The states that a caller has an address of may be changed: the gradient is that of the states that were computed."""
     e, r = gpu_engine, rng(52)
