@@ -352,7 +352,8 @@ rt_status rt_lstm_sequence_backward(rt_ctx* ctx, const float* saved, const float
  * h [steps*batch, hidden]; with one timestep h may be h0 (the state of a model that generates, updated in place), or f or v if ld = hidden.  f = +inf keeps the state
  * (padding at a sequence's end), f = -inf takes v alone (a sequence's first timestep among others), if state and v are finite.
  * Backward, from h and dh = the gradient of every h_t: df, dv with rows ldd apart, dh0 [batch, hidden] or NULL.  Otherwise results must not overlap
- * what is read, nor one another. */
+ * what is read, nor one another.  Blocks that share a long sequence wait for one another like those of rt_lstm_sequence (rt_lstm_sequence_polls):
+ * if a wait runs out, what the call writes is of no use. */
 rt_status rt_gated_scan(rt_ctx* ctx, const float* f, const float* v, int64_t ld, const float* h0, int64_t steps, int64_t batch, int64_t hidden, float* h);
 rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, int64_t ld, const float* h0, const float* h, const float* dh, int64_t steps,
                                  int64_t batch, int64_t hidden, float* df, float* dv, int64_t ldd, float* dh0);

@@ -41,6 +41,7 @@ struct ScanArgs {
   int64_t ldd;
   float* dh0;
   int* status;
+  uint32_t polls;  // looks at what another block of the cluster has not sent yet
 };
 // sigmoid(f) and 1 - sigmoid(f), each to the last bits: the smaller one is not the difference of two near ones.  1 + e lies in [1, 2], where the
 // approximate reciprocal is within one unit of the last place and a division of its own is not needed.
@@ -124,7 +125,9 @@ struct Exchange {
   float2 of_warp[2][kMaxWarps][32];             // A and B, turn by turn: a warp may be one ahead of another that still reads
   float2 of_block[2][kMaxCluster][32];          // of the cluster's blocks, turn by turn
   uint64_t arrived[2];                          // barriers that count the bytes of those
+  int gave_up[2];                               // whether a wait of such a turn ran out
 };
+__device__ __forceinline__ int volatile_load(const int* p) { return *const_cast<const volatile int*>(p); }
 template <int V>
 struct Vec;
 template <>
@@ -147,6 +150,7 @@ __device__ __forceinline__ void begin_exchange(Exchange& x) {
   if (threadIdx.x == 0) {
     tc::mbar_init(tc::smem_u32(&x.arrived[0]), 1);
     tc::mbar_init(tc::smem_u32(&x.arrived[1]), 1);
+    x.gave_up[0] = x.gave_up[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   cg::this_cluster().sync();
@@ -161,9 +165,9 @@ __device__ __forceinline__ void send(const float2* place, const uint64_t* barrie
       "r"(tc::smem_u32(barrier)), "r"(to), "f"(a), "f"(b)
       : "memory");
 }
-// Until this turn's bytes are there, which other blocks of the cluster have written; bounded.
-__device__ __forceinline__ void receive(const uint64_t* barrier, uint32_t parity, int* status) {
-  for (uint32_t i = 0; i < tc::kSpinLimit; ++i) {
+// Until this turn's bytes are there, which other blocks of the cluster have written; false if they are not after so many looks.
+__device__ __forceinline__ bool receive(const uint64_t* barrier, uint32_t parity, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -172,14 +176,24 @@ __device__ __forceinline__ void receive(const uint64_t* barrier, uint32_t parity
         : "=r"(ok)
         : "r"(tc::smem_u32(barrier)), "r"(parity)
         : "memory");
-    if (ok) return;
+    if (ok) return true;
   }
-  tc::record_status(status, 82);
+  return false;
+}
+// Nobody leaves while another block may still send to it.  Where a wait has run out, what was sent may not have landed: that takes microseconds.
+__device__ __forceinline__ void end_exchange(const Exchange& x) {
+  __syncthreads();
+  if (volatile_load(&x.gave_up[0]) | volatile_load(&x.gave_up[1])) {
+    const long long from = clock64();
+    while (clock64() - from < 2000000) {
+    }
+  }
+  cg::this_cluster().sync();
 }
 // From the A and B of this thread's timesteps to the state that they start from.  `state`: of column `lane` before the cluster's stretch, afterwards
-// before its next one.
+// before its next one.  False in all of a block if a wait of the turn before ran out: its barrier may be used no more.
 template <int C, int V, bool CLUSTER>
-__device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const float (&b)[V], int blocks, int rank, int turn, int* status, float& state,
+__device__ __forceinline__ bool start_of(Exchange& x, const float (&a)[V], const float (&b)[V], int blocks, int rank, int turn, const ScanArgs& s, float& state,
                                          float (&from)[V]) {
   constexpr int kLanes = C / V, kUnits = 32 / kLanes;  // lanes of a unit, units of a warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, unit = lane / kLanes;
@@ -211,6 +225,7 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
     for (int j = 0; j < V; ++j) x.of_warp[turn & 1][warp][lane % kLanes * V + j] = make_float2(pa[j], pb[j]);
   }
   __syncthreads();
+  if (CLUSTER && volatile_load(&x.gave_up[(turn - 1) & 1])) return false;  // which this turn does not write
   // from here on the lane is the column (lanes beyond C: nobody asks for theirs)
   float wa = 1.f, wb = 0.f, ba = 1.f, bb = 0.f;  // of the warps before this one, of all
   for (int w = 0; w < warps; ++w) {
@@ -227,7 +242,10 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
     const int slot = turn & 1;
     if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&x.arrived[slot]), blocks * 32 * (uint32_t)sizeof(float2));
     for (int to = warp; to < blocks; to += warps) send(&x.of_block[slot][rank][lane], &x.arrived[slot], to, ba, bb);
-    receive(&x.arrived[slot], turn >> 1 & 1, status);
+    if (!receive(&x.arrived[slot], turn >> 1 & 1, s.polls)) {
+      *const_cast<volatile int*>(&x.gave_up[slot]) = 1;
+      tc::record_status(s.status, 82);
+    }
     for (int r = 0; r < blocks; ++r) {
       if (r == rank) before = state;
       const float2 q = x.of_block[slot][r][lane];
@@ -239,6 +257,7 @@ __device__ __forceinline__ void start_of(Exchange& x, const float (&a)[V], const
   before = wa * before + wb;
 #pragma unroll
   for (int j = 0; j < V; ++j) from[j] = ea[j] * __shfl_sync(0xffffffffu, before, lane % kLanes * V + j) + eb[j];
+  return true;
 }
 
 template <int C, int V, int S, bool CLUSTER>
@@ -308,7 +327,7 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
     v += all * step;
     if (CLUSTER && t0 + all < s.steps) load();
     float from[V];
-    start_of<C, V, CLUSTER>(x, a[S - 1], b[S - 1], blocks, rank, turn, s.status, state, from);
+    if (!start_of<C, V, CLUSTER>(x, a[S - 1], b[S - 1], blocks, rank, turn, s, state, from)) break;
     float* ph = h;
 #pragma unroll
     for (int k = 0; k < S; ++k, ph += columns) {
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
     }
     h += all * columns;
   }
-  if (CLUSTER) cg::this_cluster().sync();  // nobody leaves while another may still send to it
+  if (CLUSTER) end_exchange(x);
 }
 
 // The same against time, for e_t = a_t d_t = a_t e_{t+1} + a_t dh_t, from which d_t = dh_t + e_{t+1}.
@@ -402,7 +421,7 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
     g -= all * columns;
     if (CLUSTER && t0 + all < s.steps) load();
     float from[V];
-    start_of<C, V, CLUSTER>(x, ea, eb, blocks, rank, turn, s.status, state, from);
+    if (!start_of<C, V, CLUSTER>(x, ea, eb, blocks, rank, turn, s, state, from)) break;
     float *pf = df, *pv = dv;
 #pragma unroll
     for (int k = 0; k < S; ++k, pf -= step_out, pv -= step_out) {
@@ -420,7 +439,7 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
     df -= all * step_out;
     dv -= all * step_out;
   }
-  if (CLUSTER) cg::this_cluster().sync();
+  if (CLUSTER) end_exchange(x);
   if (s.dh0 && rank == 0 && threadIdx.x < C && col0 + lane < columns) s.dh0[col0 + lane] = state;
 }
 
@@ -576,6 +595,7 @@ rt_status rt_gated_scan(rt_ctx* ctx, const float* f, const float* v, int64_t ld,
   s.hidden = hidden;
   s.h = h;
   s.status = ctx->device_status;
+  s.polls = ctx->sequence_polls;
   if (steps > kAhead) return aligned(s) ? launch_forward<4, 4>(ctx, s) : launch_forward<1, 16>(ctx, s);
   rt_launch(ctx, scan_columns_kernel, (unsigned)((batch * hidden + kThreads - 1) / kThreads), kThreads, 0, s);
   RT_LAUNCHED(ctx);
@@ -620,6 +640,7 @@ rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, in
   s.ldd = ldd;
   s.dh0 = dh0;
   s.status = ctx->device_status;
+  s.polls = ctx->sequence_polls;
   if (steps > kAhead) return aligned(s) ? launch_backward<4, 2>(ctx, s) : launch_backward<1, 8>(ctx, s);
   rt_launch(ctx, scan_columns_backward_kernel, (unsigned)((batch * hidden + kThreads - 1) / kThreads), kThreads, 0, s);
   RT_LAUNCHED(ctx);
