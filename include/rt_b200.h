@@ -350,7 +350,8 @@ rt_status rt_lstm_sequence_backward(rt_ctx* ctx, const float* saved, const float
 /* Gated linear recurrence over a sequence, time-major (no counterpart in the reference): a_t = sigmoid(f_t), h_t = a_t h_{t-1} + (1 - a_t) v_t.
  * f, v: [steps*batch, hidden] with rows ld floats apart: two matrices, or two column blocks of one.  h0 [batch, hidden] or NULL for zeros;
  * h [steps*batch, hidden]; with one timestep h may be h0 (the state of a model that generates, updated in place), or f or v if ld = hidden.  f = +inf keeps the state
- * (padding at a sequence's end), f = -inf takes v alone (a sequence's first timestep among others), if state and v are finite.
+ * (padding at a sequence's end), f = -inf takes v alone (a sequence's first timestep among others), if state and v are finite;
+ * an infinite state stays infinite while the gates are above zero.
  * Backward, from h and dh = the gradient of every h_t: df, dv with rows ldd apart, dh0 [batch, hidden] or NULL.  Otherwise results must not overlap
  * what is read, nor one another.  Blocks that share a long sequence wait for one another like those of rt_lstm_sequence (rt_lstm_sequence_polls):
  * if a wait runs out, what the call writes is of no use. */

@@ -9,7 +9,7 @@
 // Timesteps in a row are one timestep: from state h they lead to A h + B, with A the product of the gates.  So the sequence is walked through in
 // stretches.  The threads have some columns and timesteps each, units of lanes, warps and the blocks of a cluster one stretch after
 // the other; they tell one another their A and B (shuffles, shared memory, the cluster's), after which every thread knows the state
-// that it starts from and all of its outputs are a multiply-add each.  Everything is read and written once; the loads of the next stretch
+// that it starts from and its timesteps are a multiply-add each.  Everything is read and written once; the loads of the next stretch
 // are in flight meanwhile, or those of other blocks.  What is added in which order depends on the sizes alone.
 //
 // Bound by memory, 12 bytes an element forward and 24 backward, and near that by the instructions (about 40 and 60 an element; 88 backward
@@ -53,6 +53,9 @@ __device__ __forceinline__ void gate(float f, float& a, float& rest) {
   a = f < 0.f ? small : large;
   rest = f < 0.f ? large : small;
 }
+// A product of gates, of which `least` is the smallest, is not zero unless that is: an infinite state stays infinite, as it does timestep by timestep.
+// What that adds is 2^-149 of a state, half of which a product down there is off by anyway.
+__device__ __forceinline__ float not_lost(float product, float least) { return fmaxf(product, fminf(least, 0x1p-149f)); }
 
 // A thread has a column and walks through the sequence, the loads of eight timesteps in flight.
 __global__ void __launch_bounds__(kThreads) scan_columns_kernel(const ScanArgs s) {
@@ -207,7 +210,7 @@ __device__ __forceinline__ bool start_of(Exchange& x, const float (&a)[V], const
       const float qa = __shfl_up_sync(0xffffffffu, pa[j], o), qb = __shfl_up_sync(0xffffffffu, pb[j], o);
       if (lane >= o) {
         pb[j] = pa[j] * qb + pb[j];
-        pa[j] = pa[j] * qa;
+        pa[j] = not_lost(pa[j] * qa, fminf(pa[j], qa));
       }
     }
     ea[j] = 1.f;
@@ -235,7 +238,7 @@ __device__ __forceinline__ bool start_of(Exchange& x, const float (&a)[V], const
     }
     const float2 q = x.of_warp[turn & 1][w][lane];
     bb = q.x * bb + q.y;
-    ba = q.x * ba;
+    ba = not_lost(q.x * ba, fminf(q.x, ba));
   }
   float before = state;
   if (CLUSTER) {
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
   int turn = 0;
   for (int64_t t0 = 0; t0 < s.steps; t0 += all, ++turn) {
     if (!CLUSTER) load();
-    float a[S][V], b[S][V];  // from the thread's first timestep on
+    float a[S][V], b[S][V], all_a[V], all_b[V], least[V];  // of each timestep; of the thread's together
 #pragma unroll
     for (int k = 0; k < S; ++k)
 #pragma unroll
@@ -316,24 +319,25 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
         float rest;
         gate(fs[k][j], a[k][j], rest);
         b[k][j] = rest * vs[k][j];
-        if (k > 0) {
-          b[k][j] += a[k][j] * b[k - 1][j];
-          a[k][j] *= a[k - 1][j];
-        }
+        all_b[j] = k > 0 ? a[k][j] * all_b[j] + b[k][j] : b[k][j];
+        all_a[j] = k > 0 ? a[k][j] * all_a[j] : a[k][j];
+        least[j] = k > 0 ? fminf(a[k][j], least[j]) : a[k][j];
       }
+#pragma unroll
+    for (int j = 0; j < V; ++j) all_a[j] = not_lost(all_a[j], least[j]);
     const int mine = left;
     t += all;
     f += all * step;
     v += all * step;
     if (CLUSTER && t0 + all < s.steps) load();
     float from[V];
-    if (!start_of<C, V, CLUSTER>(x, a[S - 1], b[S - 1], blocks, rank, turn, s, state, from)) break;
+    if (!start_of<C, V, CLUSTER>(x, all_a, all_b, blocks, rank, turn, s, state, from)) break;
     float* ph = h;
 #pragma unroll
     for (int k = 0; k < S; ++k, ph += columns) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) b[k][j] += a[k][j] * from[j];
-      if (k < mine) Vec<V>::store(ph, b[k]);
+      for (int j = 0; j < V; ++j) from[j] = a[k][j] * from[j] + b[k][j];
+      if (k < mine) Vec<V>::store(ph, from);
     }
     h += all * columns;
   }
@@ -395,24 +399,20 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
   int turn = 0;
   for (int64_t t0 = 0; t0 < s.steps; t0 += all, ++turn) {
     if (!CLUSTER) load();
-    float da[S][V], db[S][V], slope[S][V], rest[S][V], ea[V], eb[V];  // d = da * (e behind the thread's timesteps) + db
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      ea[j] = 1.f;
-      eb[j] = 0.f;
-    }
+    float a[S][V], g_now[S][V], slope[S][V], rest[S][V], all_a[V], all_b[V], least[V];  // of each timestep; of the thread's together: e, from e behind them
 #pragma unroll
     for (int k = 0; k < S; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float a;
-        gate(fs[k][j], a, rest[k][j]);
-        slope[k][j] = (hs[k][j] - vs[k][j]) * a * rest[k][j];
-        da[k][j] = ea[j];
-        db[k][j] = gs[k][j] + eb[j];
-        ea[j] = a * da[k][j];
-        eb[j] = a * db[k][j];
+        gate(fs[k][j], a[k][j], rest[k][j]);
+        slope[k][j] = (hs[k][j] - vs[k][j]) * a[k][j] * rest[k][j];
+        g_now[k][j] = gs[k][j];
+        all_b[j] = a[k][j] * (k > 0 ? gs[k][j] + all_b[j] : gs[k][j]);
+        all_a[j] = k > 0 ? a[k][j] * all_a[j] : a[k][j];
+        least[j] = k > 0 ? fminf(a[k][j], least[j]) : a[k][j];
       }
+#pragma unroll
+    for (int j = 0; j < V; ++j) all_a[j] = not_lost(all_a[j], least[j]);
     const int mine = left;
     t -= all;
     f -= all * step;
@@ -421,15 +421,16 @@ __global__ void __launch_bounds__(32 * (CLUSTER ? kMaxWarps : kAloneWarps), CLUS
     g -= all * columns;
     if (CLUSTER && t0 + all < s.steps) load();
     float from[V];
-    if (!start_of<C, V, CLUSTER>(x, ea, eb, blocks, rank, turn, s, state, from)) break;
+    if (!start_of<C, V, CLUSTER>(x, all_a, all_b, blocks, rank, turn, s, state, from)) break;
     float *pf = df, *pv = dv;
 #pragma unroll
     for (int k = 0; k < S; ++k, pf -= step_out, pv -= step_out) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = da[k][j] * from[j] + db[k][j];
+        const float d = g_now[k][j] + from[j];
         slope[k][j] *= d;
         rest[k][j] *= d;
+        from[j] = a[k][j] * d;
       }
       if (k < mine) {
         Vec<V>::store(pf, slope[k]);
