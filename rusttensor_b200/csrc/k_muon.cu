@@ -202,8 +202,10 @@ struct Product {
   float* sums;           // partial sums of tiles, [columns][128 rows] each
   unsigned* tickets;     // zero
   unsigned* arrived;     // zero; blocks that have done their part, of all products
+  uint32_t polls;        // looks at that for each product
   int* status;
 };
+constexpr unsigned kGaveUp = 1u << 31;  // in `arrived`: a wait has run out somewhere
 // Results are finished by slabs of 64 columns.
 constexpr int kSlab = 64;
 // A tile of W columns has 128 rows and belongs to a CTA, or (PAIR) 256 rows and belongs to two CTAs of a cluster: each has 128 of the rows and
@@ -579,7 +581,7 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
       asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
       if (threadIdx.x == 0) {
         unsigned* ticket = p.tickets + (p.item[t.q].first_ticket[phase] + t.index << PAIR) + acc.rank;
-        const int d = (int)atomicAdd(ticket, 1u);
+        const int d = *acc.abort ? -1 : (int)atomicAdd(ticket, 1u);  // with a share missing, nobody finishes the tile
         if (d == splits - 1) *ticket = 0;
         *acc.drawn = d;
       }
@@ -608,10 +610,12 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
           *reinterpret_cast<float4*>(acc.slab + piece_at(acc.quad * 32 + acc.lane, (acc.group * cols % kSlab + j) / 4)) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
       }
       asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+      const int out = *acc.abort ? 1 << 30 : 0;  // if a wait has run out, results lie outside
+      slab.c += out;
       slab.rows(q, from, acc.slab, row0);
       if (Slab<PHASE>::kSymmetric || (PHASE == kResult && q.tall)) {
         asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
-        slab.columns(q, acc.slab, row0, col0, warp, acc.lane);
+        slab.columns(q, acc.slab, row0 + out, col0, warp, acc.lane);
       }
       asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
     }
@@ -625,7 +629,9 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
 // (some 37 bytes a cycle and SM): a pair with W = 256 takes 64 KB a K-block and CTA for 128 x 256 results, one CTA alone would take 96.
 // Between two products a block's warps count the block as done when they have written their results, and its TMA warp waits for all blocks
 // before it brings in what the next product reads and lets the block's others go on.  Every wait is bounded; on expiry the kernel records
-// a code in the status word, raises a flag that all other waits poll, lets its own copies land, frees tensor memory and returns.
+// a code in the status word, raises a flag that all other waits poll, lets its own copies land, frees tensor memory and returns.  From then on the
+// block writes no result and does not count as done, so that no other one goes on to the next product: `out`, which the last one writes, is
+// what it was unless the wait was that one's.
 template <int W, bool PAIR>
 __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_kernel(const __grid_constant__ Product p) {
   using M = Layout<W, PAIR>;
@@ -670,10 +676,10 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
         if (product > 0) {
           const unsigned all = gridDim.x * (unsigned)product;
           unsigned there = 0;
-          for (uint32_t k = 0; k < kSpinLimit && there < all && !*abort_flag; ++k)
+          for (uint32_t k = 0; k < p.polls && there < all && !*abort_flag; ++k)
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.arrived) : "memory");
-          if (there < all) {
-            if (!*abort_flag) record_status(p.status, 97);
+          if (there < all || there >= kGaveUp) {
+            if (there < all && !*abort_flag) record_status(p.status, 97);
             *abort_flag = 1;
             ok = false;
             break;
@@ -702,6 +708,7 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
           }
         }
       }
+      if (!ok) asm volatile("red.relaxed.gpu.global.or.b32 [%0], %1;" ::"l"(p.arrived), "r"(kGaveUp) : "memory");
       // what the MMA warp tells of the last stages has arrived before the CTA may leave, and copies that nobody has waited for have landed
       for (int i = it > kStages ? it - kStages : 0; ok && i < it; ++i) ok = parts::wait(empty(i % kStages), (i / kStages) & 1, p.status, 99, abort_flag);
       if (!ok && rank == 0)
@@ -778,7 +785,7 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
         else finish_tiles<kResult, W, PAIR>(p, acc, step & 1);
         if (product + 1 == 3 * p.steps) break;
         asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
-        if (threadIdx.x == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.arrived) : "memory");
+        if (threadIdx.x == 0 && !*abort_flag) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.arrived) : "memory");
       }
     }
   }
@@ -954,6 +961,7 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
   Parts x{};
   p.count = x.count = count;
   p.status = ctx->device_status;
+  p.polls = ctx->sequence_polls;
   size_t halves = 0, at[kGroup];
   for (int q = 0; q < count; ++q) {
     Item& i = p.item[q];

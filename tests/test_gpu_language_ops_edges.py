@@ -7,7 +7,7 @@ import pytest
 import language_ref as ref
 import rusttensor_b200
 from helpers import rng
-from test_gpu_language_ops import i64
+from test_gpu_language_ops import as_near_as_fp32, f32, i64, matrix, pointers, steps_on_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,29 @@ def test_gated_scan_forgets_entirely(capi):
     d = [capi.to_device(a) for a in (f, v)]
     capi.call("gated_scan", d[0].ptr, d[1].ptr, i64(hidden), h0.ptr, i64(steps), i64(1), i64(hidden), h.ptr)
     assert np.all(h.numpy()[250:] == 0)
+
+
+@pytest.mark.parametrize("shapes", [[(784, 128), (128, 10)], [(2000, 70)], [(1501, 1603)], [(1290, 1803)] * 5], ids=lambda s: f"{len(s)}x{s[0][0]}x{s[0][1]}")
+def test_a_wait_of_muon_that_runs_out(shapes):
+    """Blocks that do not wait for one another between two products: the kernel ends, the next synchronising call says so, and the parameters are as
+    they were; the calls after it are right."""
+    import torch
+
+    api, r = rusttensor_b200.CApi(), rng(69)
+    host, ones = [matrix(r, s) for s in shapes], [np.ones(s, np.float32) for s in shapes]
+    g, m, p = ([api.to_device(x) for x in xs] for xs in (host, [0 * x for x in ones], ones))
+    args = (len(shapes), pointers(p), pointers(g), pointers(m), api.i64([s[0] for s in shapes]), api.i64([s[1] for s in shapes]))
+    api.call("lstm_sequence_polls", i64(0))
+    api.call("muon_step_multi", *args, f32(-1.0), f32(0.0), 0, f32(0.0), 5, f32(1.0))
+    code = C.c_int(0)
+    with pytest.raises(Exception, match="gave up"):
+        api.call("device_status", C.byref(code))
+    assert code.value == 97
+    api.call("device_status", C.byref(code))
+    assert code.value == 0
+    assert all(np.array_equal(x.numpy(), one) for x, one in zip(p, ones))
+    api.call("lstm_sequence_polls", i64(-1))
+    api.call("orthogonalize_list", len(shapes), pointers(g), *args[4:], 5, pointers(p))
+    for x, d in zip(host, p):
+        as_near_as_fp32(d.numpy(), steps_on_gpu(x, torch.float64), steps_on_gpu(x, torch.float32))
+    api.close()
