@@ -8,10 +8,14 @@
 //
 // A step is three products, each of which has to wait for the one before: G = X X^T and b G + c G^2, both symmetric, of which the lower half is
 // computed and written twice, and a X + (b G + c G^2) X.  Errors of early steps grow (small singular values by 3.4 a step), so the products
-// keep fp32's precision: an operand is held as two fp16 parts, hi = fp16(2^12 x) and lo = fp16(2^12 x - hi), 22 bits, and a product is three
-// tcgen05.mma of kind::f16: hi lo, lo hi and hi hi.  No element of X, G or the polynomial is beyond 3 (their singular values are at most 1.21,
-// 1.46 and 2.81), so the scale is fixed and nothing is looked at beforehand; below 2^-15, where lo has fewer than 11 bits left, an element is
-// off by 2^-37 at most.  A product's epilogue adds what
+// keep fp32's precision: an operand is held as two fp16 parts, hi = fp16(2^15 x) and lo = fp16(2^15 x - hi), 22 bits, and a product is three
+// tcgen05.mma of kind::f16: hi lo, lo hi and hi hi.  No element of X, G or the polynomial is beyond 1.21, 1.46 and 2.81 (bounds of their singular
+// values; the polynomial takes 2^14), so the scale is fixed.  Below 2^-18, where lo has fewer than 11 bits left, an element is off by
+// 2^-40 at most, which is 2^-20 of a row or column of k elements as long as its norm is sqrt(k) 2^-20 or more: rows whose norms differ by exp(N(0, 1)), as in
+// 4096 x 4096, stay above that.  Where a row or a column that is not zero lies below, the matrix is wide: its operands are three bf16 parts, 24
+// bits of fp32's range, and a product is six MMAs (all but the three smallest), so that every row and column is as near as in fp32 against its own
+// size: what a step adds up for one has that size as a factor.  (With two parts rows 2^-16 of the others were 9e-5 off and rows 2^-32 of them not updated
+// at all.)  Rows and columns shrink by no more than a factor of ten over all steps, so this is decided once.  A product's epilogue adds what
 // the formula adds and writes the parts that the next product reads, as they lie: X [m][n] is an operand with n as the reduction, and with
 // m, by tensor maps and MMA descriptors of either kind.  All matrices of a call go through every product together, and all products are one
 // cooperative launch, whose blocks wait for one another between two products (15 launches for five steps were 4 us each besides the work).
@@ -20,7 +24,10 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 #include <vector>
+
+#include <cuda_bf16.h>
 
 #include "parts_common.cuh"
 
@@ -49,6 +56,8 @@ struct Squares {
   Update u[kGroup];
   int64_t n[kGroup];
   double* sums;  // [matrix][block]
+  unsigned long long* zero;  // what later launches begin with zeros
+  int64_t zeros;
 };
 template <bool VEC>
 __device__ __forceinline__ double sum_of_squares(const Update& u, int64_t n) {
@@ -99,6 +108,7 @@ __device__ __forceinline__ double sum_of_squares(const Update& u, int64_t n) {
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Squares p) {
   RT_PDL_ENTRY();
   __shared__ double of_warp[kThreads / 32];
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < p.zeros; i += (int64_t)gridDim.x * kThreads) p.zero[i] = 0;
   const int q = blockIdx.x / kNormBlocks;
   const Update u = p.u[q];
   const int64_t n = p.n[q];
@@ -158,13 +168,15 @@ struct Matrix {
   float keep, step;
 };
 
-rt_status launch_squares(rt_ctx* ctx, const Matrix* list, int count, double* sums) {
+rt_status launch_squares(rt_ctx* ctx, const Matrix* list, int count, double* sums, unsigned long long* zero = nullptr, int64_t zeros = 0) {
   Squares p{};
   for (int q = 0; q < count; ++q) {
     p.u[q] = list[q].u;
     p.n[q] = list[q].rows * list[q].cols;
   }
   p.sums = sums;
+  p.zero = zero;
+  p.zeros = zeros;
   rt_launch(ctx, squares_kernel, kNormBlocks * count, kThreads, 0, p);
   RT_LAUNCHED(ctx);
   return RT_OK;
@@ -175,7 +187,8 @@ using namespace tc;
 namespace cg = cooperative_groups;
 using parts::kBox;
 
-constexpr float kScale = 4096.f;
+constexpr float kScale = 32768.f, kScaleS = 16384.f;  // of the two parts of X and G; of the polynomial
+constexpr int kPlanes = 3;
 constexpr int kTileM = 128, kBlockK = 64;  // rows of a tile; elements of the reduction that a stage holds
 constexpr uint32_t kSecond = 256;          // tensor-memory column of the second accumulator
 enum { kGram, kSquare, kApply, kResult };  // kResult: the last kApply, whose result goes to `out`
@@ -183,7 +196,7 @@ enum { kGram, kSquare, kApply, kResult };  // kResult: the last kApply, whose re
 struct Item {
   int m, n;              // m <= n
   int ldx, ldm;          // halves between rows of X, of G and the polynomial
-  uint16_t *x[2], *g, *s;
+  uint16_t *x[2], *g, *s; // kPlanes each: hi, lo; or, of a wide matrix, the middle one, the first, the last.  X begins in x[0], of a wide matrix in x[1]
   int first[3], splits[3];  // by product: first work item of the matrix, CTAs that share a tile's reduction
   int first_part[3];        // partial sums of the matrices before, in tiles
   int first_ticket[3];
@@ -193,12 +206,13 @@ struct Item {
   float keep, step;
 };
 struct Product {
-  // X, G and the polynomial, both planes in a box: 128 rows high as left operands, as right ones as many as a CTA brings in, X 64 as the right operand
+  // X, G and the polynomial, two planes in a box: 128 rows high as left operands, as right ones as many as a CTA brings in, X 64 as the right operand
   // whose rows are the reduction.
   CUtensorMap x_left[2][kGroup], x_right[2][kGroup], x_apply[2][kGroup], g_left[kGroup], g_right[kGroup], s_left[kGroup];
   Item item[kGroup];
   int count, steps;
   int items[3];
+  const unsigned* wide;  // a bit for each matrix
   float* sums;           // partial sums of tiles, [columns][128 rows] each
   unsigned* tickets;     // zero
   unsigned* arrived;     // zero; blocks that have done their part, of all products
@@ -228,9 +242,9 @@ struct Tile {
 };
 // K-blocks that an accumulator sums before it is emptied into registers, because it adds with truncation.  After two a long reduction is nearer to the
 // exact result than one in fp32 (five steps of 4096 x 4096: 1.6e-6 and 4.9e-6 off); a short one needs the half of that (784 x 128: 1.7e-6, 1.6e-6 in
-// fp32), where it costs little.
+// fp32), where it costs little.  Wide matrices take one, whose small products come first.
 template <int W>
-__device__ __forceinline__ int chunk_of(int depth) { return W == 64 && depth < 1024 ? 1 : 2; }
+__device__ __forceinline__ int chunk_of(int depth, bool wide) { return wide || (W == 64 && depth < 1024) ? 1 : 2; }
 template <int W, bool PAIR>
 __device__ __forceinline__ Tile tile_of(const Product& p, int phase, int i) {
   constexpr int rows = Layout<W, PAIR>::rows;
@@ -397,9 +411,9 @@ __device__ __forceinline__ void mma_one(uint32_t d, uint32_t a, uint32_t b, uint
     parts::mma(d, a, desc_hi, b, desc_hi, idesc, more);
 }
 // Two neighbouring values as parts.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  a *= kScale;
-  b *= kScale;
+__device__ __forceinline__ void split2(float a, float b, float scale, uint32_t& hi, uint32_t& lo) {
+  a *= scale;
+  b *= scale;
   const __half2 h = __floats2half2_rn(a, b);
   const float2 back = __half22float2(h);
   const __half2 l = __floats2half2_rn(a - back.x, b - back.y);
@@ -409,6 +423,25 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 __device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi)), l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
   return make_float2((h.x + l.x) * (1.f / kScale), (h.y + l.y) * (1.f / kScale));
+}
+__device__ __forceinline__ float2 of_bf16(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t to_bf16(float2& v) {  // leaves the rest
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+  const float2 back = of_bf16(w);
+  v.x -= back.x;
+  v.y -= back.y;
+  return w;
+}
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[kPlanes]) {
+  float2 v = make_float2(a, b);
+  w[1] = to_bf16(v);
+  w[0] = to_bf16(v);
+  w[2] = to_bf16(v);
+}
+__device__ __forceinline__ float2 join3(uint32_t middle, uint32_t first, uint32_t last) {
+  const float2 m = of_bf16(middle), h = of_bf16(first), l = of_bf16(last);
+  return make_float2(h.x + m.x + l.x, h.y + m.y + l.y);
 }
 // A CTA's 128 x 64 results in shared memory, four columns a piece; where a row has its pieces keeps apart what is accessed together: the same
 // piece of eight rows in a row, and of every fourth one.
@@ -420,6 +453,7 @@ __device__ __forceinline__ int piece_at(int row, int piece) { return row * kSlab
 template <int PHASE>
 struct Slab {
   static constexpr bool kSymmetric = PHASE == kGram || PHASE == kSquare;
+  static constexpr float kOut = PHASE == kSquare ? kScaleS : kScale;
   int r, c;  // the lane's first row and column of eight; its second row is four behind
   uint4 hi[2], lo[2];
   __device__ __forceinline__ Slab(int row, int col, int warp, int lane) : r(row + warp * 8 + (lane >> 3)), c(col + (lane & 7) * 8) {}
@@ -441,7 +475,7 @@ struct Slab {
     }
   }
   // What is added has been fetched; the sums are in the slab.  row0, col0: of the slab.
-  __device__ __forceinline__ void rows(const Item& q, int from, float* slab, int row0) {
+  __device__ __forceinline__ void rows(const Item& q, int from, bool wide, float* slab, int row0) {
     const int ld = kSymmetric ? q.ldm : q.ldx;
     uint16_t* to = (PHASE == kGram ? q.g : (PHASE == kSquare ? q.s : (from ? q.x[0] : q.x[1]))) + (int64_t)r * ld + c;
     const int64_t plane = (int64_t)q.m * ld;
@@ -452,16 +486,32 @@ struct Slab {
       float4* at[2] = {reinterpret_cast<float4*>(slab + piece_at(y, piece)), reinterpret_cast<float4*>(slab + piece_at(y, piece + 1))};
       const float4 s0 = *at[0], s1 = *at[1];
       float v[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-      constexpr float f = (PHASE == kSquare ? kC : 1.f) / (kScale * kScale), g = PHASE == kSquare ? kB : kA;
-      const uint32_t hs[4] = {hi[k].x, hi[k].y, hi[k].z, hi[k].w}, ls[4] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w};
+      constexpr float f = PHASE == kSquare ? kC : 1.f, g = PHASE == kSquare ? kB : kA, scale = kScale * (PHASE == kGram || PHASE == kSquare ? kScale : kScaleS);
+      if (!wide) {
+        const uint32_t hs[4] = {hi[k].x, hi[k].y, hi[k].z, hi[k].w}, ls[4] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] *= f;
-        v[2 * j + 1] *= f;
-        if (PHASE != kGram) {
-          const float2 w = join2(hs[j], ls[j]);
-          v[2 * j] += g * w.x;
-          v[2 * j + 1] += g * w.y;
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] *= f / scale;
+          v[2 * j + 1] *= f / scale;
+          if (PHASE != kGram) {
+            const float2 w = join2(hs[j], ls[j]);
+            v[2 * j] += g * w.x;
+            v[2 * j + 1] += g * w.y;
+          }
+        }
+      } else if (PHASE != kGram && in(q, k)) {
+        const uint16_t* more = (PHASE == kSquare ? q.g : (from ? q.x[1] : q.x[0])) + (int64_t)(r + 4 * k) * ld + c;
+        uint32_t parts[kPlanes][4];
+#pragma unroll
+        for (int i = 0; i < kPlanes; ++i) {
+          const uint4 w = __ldcg(reinterpret_cast<const uint4*>(more + i * plane));
+          parts[i][0] = w.x; parts[i][1] = w.y; parts[i][2] = w.z; parts[i][3] = w.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 w = join3(parts[0][j], parts[1][j], parts[2][j]);
+          v[2 * j] = f * v[2 * j] + g * w.x;
+          v[2 * j + 1] = f * v[2 * j + 1] + g * w.y;
         }
       }
       if (turned) {
@@ -474,19 +524,25 @@ struct Slab {
           put(q, o, make_float4(v[0], v[1], v[2], v[3]), q.n - c);
           put(q, o + 4, make_float4(v[4], v[5], v[6], v[7]), q.n - c - 4);
         }
-      } else if (in(q, k)) {
+      } else if (in(q, k) && !wide) {
         uint4 h, l;
-        split2(v[0], v[1], h.x, l.x);
-        split2(v[2], v[3], h.y, l.y);
-        split2(v[4], v[5], h.z, l.z);
-        split2(v[6], v[7], h.w, l.w);
+        split2(v[0], v[1], kOut, h.x, l.x);
+        split2(v[2], v[3], kOut, h.y, l.y);
+        split2(v[4], v[5], kOut, h.z, l.z);
+        split2(v[6], v[7], kOut, h.w, l.w);
         *reinterpret_cast<uint4*>(to + (int64_t)4 * k * ld) = h;
         *reinterpret_cast<uint4*>(to + (int64_t)4 * k * ld + plane) = l;
+      } else if (in(q, k)) {
+        uint32_t w[4][kPlanes];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split3(v[2 * j], v[2 * j + 1], w[j]);
+#pragma unroll
+        for (int i = 0; i < kPlanes; ++i) *reinterpret_cast<uint4*>(to + (int64_t)4 * k * ld + i * plane) = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
       }
     }
   }
   // A warp writes four columns as rows, a lane four values of each.
-  __device__ __forceinline__ void columns(const Item& q, const float* slab, int row0, int col0, int warp, int lane) {
+  __device__ __forceinline__ void columns(const Item& q, bool wide, const float* slab, int row0, int col0, int warp, int lane) {
     const int y = lane * 4, first = row0 + y, left = q.m - first, width = kSymmetric ? q.m : q.n;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -497,11 +553,20 @@ struct Slab {
       for (int j = 0; j < 4; ++j) v[j] = slab[piece_at(y + j, x >> 2) + (x & 3)];
       if (kSymmetric) {
         uint16_t* o = (PHASE == kGram ? q.g : q.s) + (int64_t)col * q.ldm + first;
-        uint2 h, l;
-        split2(v[0], v[1], h.x, l.x);
-        split2(v[2], v[3], h.y, l.y);
-        *reinterpret_cast<uint2*>(o) = h;
-        *reinterpret_cast<uint2*>(o + (int64_t)q.m * q.ldm) = l;
+        const int64_t plane = (int64_t)q.m * q.ldm;
+        if (!wide) {
+          uint2 h, l;
+          split2(v[0], v[1], kOut, h.x, l.x);
+          split2(v[2], v[3], kOut, h.y, l.y);
+          *reinterpret_cast<uint2*>(o) = h;
+          *reinterpret_cast<uint2*>(o + plane) = l;
+        } else {
+          uint32_t w[2][kPlanes];
+          split3(v[0], v[1], w[0]);
+          split3(v[2], v[3], w[1]);
+#pragma unroll
+          for (int i = 0; i < kPlanes; ++i) *reinterpret_cast<uint2*>(o + i * plane) = make_uint2(w[0][i], w[1][i]);
+        }
       } else {
         put(q, q.out + (int64_t)col * q.m + first, make_float4(v[0], v[1], v[2], v[3]), left);
       }
@@ -536,9 +601,10 @@ struct Accumulators {
   volatile int *abort, *drawn;
   float* slab;
   int quad, group, lane, rank;
+  unsigned wide;
 };
-template <int PHASE, int W, bool PAIR>
-__device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc, int from) {
+template <int PHASE, int W, bool PAIR, bool WIDE_ONES>
+__device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc, int step) {
   using M = Layout<W, PAIR>;
   constexpr int cols = M::cols;
   constexpr int phase = PHASE == kResult ? kApply : PHASE;
@@ -548,10 +614,12 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
     const int splits = p.item[t.q].splits[phase];
     const Item q = p.item[t.q];  // of its own: what is left in the parameters is read again after every store
     const int row0 = t.row + acc.rank * kTileM, warp = threadIdx.x >> 5, width = PHASE == kGram || PHASE == kSquare ? q.m : q.n;
+    const bool wide = WIDE_ONES && (acc.wide >> t.q & 1);
+    const int from = (step ^ (int)wide) & 1;
     constexpr bool early = W == 64;  // what is added is on its way during the product: elsewhere there are no registers for it
     Slab<PHASE> slab(row0, t.col, warp, acc.lane);
-    if (early) slab.fetch(q, from);
-    const int chunk = chunk_of<W>(phase == kGram ? q.n : q.m), chunks = (t.k1 - t.k0 + chunk - 1) / chunk;
+    if (early && !wide) slab.fetch(q, from);
+    const int chunk = chunk_of<W>(phase == kGram ? q.n : q.m, wide), chunks = (t.k1 - t.k0 + chunk - 1) / chunk;
     float sum[cols];
 #pragma unroll
     for (int j = 0; j < cols; ++j) sum[j] = 0.f;
@@ -602,7 +670,7 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
       if (row0 >= q.m || col0 >= width || (Slab<PHASE>::kSymmetric && col0 >= row0 + kTileM)) break;  // the same for all warps
       if (!early || k > 0) {
         slab = Slab<PHASE>(row0, col0, warp, acc.lane);
-        slab.fetch(q, from);
+        if (!wide) slab.fetch(q, from);
       }
       if (acc.group * cols / kSlab == k) {
 #pragma unroll
@@ -612,10 +680,10 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
       asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
       const int out = *acc.abort ? 1 << 30 : 0;  // if a wait has run out, results lie outside
       slab.c += out;
-      slab.rows(q, from, acc.slab, row0);
+      slab.rows(q, from, wide, acc.slab, row0);
       if (Slab<PHASE>::kSymmetric || (PHASE == kResult && q.tall)) {
         asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
-        slab.columns(q, acc.slab, row0 + out, col0, warp, acc.lane);
+        slab.columns(q, wide, acc.slab, row0 + out, col0, warp, acc.lane);
       }
       asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
     }
@@ -625,7 +693,7 @@ __device__ __forceinline__ void finish_tiles(const Product& p, Accumulators& acc
 // All products of all steps.  Roles of a CTA, one per SM, that walks over tiles: a TMA warp some K-blocks of 64 ahead, an MMA warp (of a pair's first
 // CTA), and warps that empty the accumulators into registers and write the result, 16 of them where a tile's latency counts.  Where the
 // tiles are fewer than the SMs, several CTAs share a tile's reduction: each leaves its sums in memory, and the one that draws the last ticket
-// adds them up in their order.  A K-block takes 12 MMAs.  What bounds large products otherwise is what all SMs together bring in from the L2 cache
+// adds them up in their order.  A K-block takes 12 MMAs, of a wide matrix 24 on two stages: the first and last parts, then the middle and first.  What bounds large products otherwise is what all SMs together bring in from the L2 cache
 // (some 37 bytes a cycle and SM): a pair with W = 256 takes 64 KB a K-block and CTA for 128 x 256 results, one CTA alone would take 96.
 // Between two products a block's warps count the block as done when they have written their results, and its TMA warp waits for all blocks
 // before it brings in what the next product reads and lets the block's others go on.  Every wait is bounded; on expiry the kernel records
@@ -665,130 +733,157 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  bool ok = true;
-
-  if (warp == M::tma) {
-    if (lane == 0) {
+  const unsigned wide_ones = *p.wide;
+  // Whether any matrix is wide is compiled for itself: what wide ones need would take registers from the others (five layers 457 us instead of 383).
+  auto run = [&](auto any) {
+    constexpr bool WIDE_ONES = decltype(any)::value;
+    bool ok = true;
+    if (warp == M::tma) {
+      if (lane == 0) {
+        int it = 0;
+        for (int product = 0; product < 3 * p.steps && ok; ++product) {
+          const int phase = product % 3, items = p.items[phase];
+          Tile t = tile_of<W, PAIR>(p, phase, unit);  // before the wait: a thousand cycles
+          if (product > 0) {
+            const unsigned all = gridDim.x * (unsigned)product;
+            unsigned there = 0;
+            for (uint32_t k = 0; k < p.polls && there < all && !*abort_flag; ++k)
+              asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.arrived) : "memory");
+            if (there < all || there >= kGaveUp) {
+              if (there < all && !*abort_flag) record_status(p.status, 97);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            mbar_arrive(go);
+          }
+          asm volatile("fence.proxy.async.global;" ::: "memory");  // the parts were written by ordinary stores
+          for (int i = unit; i < items && ok; i += units) {
+            if (i != unit) t = tile_of<W, PAIR>(p, phase, i);
+            const int wide = WIDE_ONES ? wide_ones >> t.q & 1 : 0, from = product / 3 + wide & 1;
+            const CUtensorMap* map_a = phase == kGram ? &p.x_left[from][t.q] : (phase == kSquare ? &p.g_left[t.q] : &p.s_left[t.q]);
+            const CUtensorMap* map_b = phase == kGram ? &p.x_right[from][t.q] : (phase == kSquare ? &p.g_right[t.q] : &p.x_apply[from][t.q]);
+            for (int kb = t.k0, z = wide; kb < t.k1 && ok; ++it) {  // from plane z on
+              const int st = it % kStages;
+              if (it >= kStages) ok = parts::wait(empty(st), (it / kStages - 1) & 1, p.status, 91, abort_flag);
+              if (!ok) break;
+              const uint32_t dst = base + st * M::stage;
+              if (rank == 0) mbar_expect_tx(full(st), M::stage << PAIR);
+              load_3d<PAIR>(dst, map_a, kb * kBlockK, t.row + rank * kTileM, z, full(st));
+              const int col = t.col + rank * M::right;
+              if (phase == kApply) {
+  #pragma unroll
+                for (int j = 0; j < M::right / 64; ++j) load_3d<PAIR>(dst + (4 + 2 * j) * kBox, map_b, col + j * 64, kb * kBlockK, z, full(st));
+              } else {
+                load_3d<PAIR>(dst + 4 * kBox, map_b, kb * kBlockK, col, z, full(st));
+              }
+              if (z == 0) {
+                ++kb;
+                z = wide;
+              } else {
+                z = 0;
+              }
+            }
+          }
+        }
+        if (!ok) asm volatile("red.relaxed.gpu.global.or.b32 [%0], %1;" ::"l"(p.arrived), "r"(kGaveUp) : "memory");
+        // what the MMA warp tells of the last stages has arrived before the CTA may leave, and copies that nobody has waited for have landed
+        for (int i = it > kStages ? it - kStages : 0; ok && i < it; ++i) ok = parts::wait(empty(i % kStages), (i / kStages) & 1, p.status, 99, abort_flag);
+        if (!ok && rank == 0)
+          for (int i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait(full(i % kStages), (i / kStages) & 1, p.status, 92);
+      }
+    } else if (warp == M::mma) {
+      if (rank == 0) {
+      // Descriptors as in parts_common.cuh: groups of 8 rows (of 8 K) 1024 bytes apart, 128-byte swizzle; where the columns lie side by side instead of
+      // the reduction, groups of 64 columns, both planes of them, 2 * kBox apart.
+      constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t lbo = (2 * kBox >> 4) << 16, slot_a = 32 >> 4;  // mma_block has the latter as 2
       int it = 0;
+      uint32_t chunks = 0;
       for (int product = 0; product < 3 * p.steps && ok; ++product) {
-        const int phase = product % 3, from = product / 3 & 1, items = p.items[phase];
-        Tile t = tile_of<W, PAIR>(p, phase, unit);  // before the wait: a thousand cycles
-        if (product > 0) {
-          const unsigned all = gridDim.x * (unsigned)product;
-          unsigned there = 0;
-          for (uint32_t k = 0; k < p.polls && there < all && !*abort_flag; ++k)
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.arrived) : "memory");
-          if (there < all || there >= kGaveUp) {
-            if (there < all && !*abort_flag) record_status(p.status, 97);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          mbar_arrive(go);
-        }
-        asm volatile("fence.proxy.async.global;" ::: "memory");  // the parts were written by ordinary stores
+        const int phase = product % 3, items = p.items[phase];
+        const uint32_t slot_b = phase == kApply ? 2048 >> 4 : 32 >> 4;
+        const uint32_t idesc_f16 = (1u << 4) | (uint32_t)(phase == kApply) << 16 | (uint32_t)(M::rows >> 4) << 24 | (uint32_t)(W >> 3) << 17;
         for (int i = unit; i < items && ok; i += units) {
-          if (i != unit) t = tile_of<W, PAIR>(p, phase, i);
-          const CUtensorMap* map_a = phase == kGram ? &p.x_left[from][t.q] : (phase == kSquare ? &p.g_left[t.q] : &p.s_left[t.q]);
-          const CUtensorMap* map_b = phase == kGram ? &p.x_right[from][t.q] : (phase == kSquare ? &p.g_right[t.q] : &p.x_apply[from][t.q]);
-          for (int kb = t.k0; kb < t.k1 && ok; ++kb, ++it) {
+          const Tile t = tile_of<W, PAIR>(p, phase, i);
+          const bool wide = WIDE_ONES && (wide_ones >> t.q & 1);
+          const int depth = phase == kGram ? p.item[t.q].n : p.item[t.q].m, chunk = chunk_of<W>(depth, wide);
+          const uint32_t idesc = idesc_f16 | (wide ? 1u << 7 | 1u << 10 : 0u);
+          for (int kb = t.k0, z = wide, in_chunk = 0; kb < t.k1 && ok; ++it) {
             const int st = it % kStages;
-            if (it >= kStages) ok = parts::wait(empty(st), (it / kStages - 1) & 1, p.status, 91, abort_flag);
+            const bool first = in_chunk == 0, last = z == 0 && (wide || in_chunk + 1 == chunk || kb + 1 == t.k1);
+            in_chunk = last ? 0 : in_chunk + 1;
+            const uint32_t a = ((base + st * M::stage) >> 4 & 0x3FFF) | lbo, b = ((base + st * M::stage + 4 * kBox) >> 4 & 0x3FFF) | lbo;
+            const uint32_t a_lo = a + (2 * kBox >> 4), b_lo = b + ((phase == kApply ? 1 : M::right / 64) * kBox >> 4), second = chunks & 1;
+            const uint32_t d = tmem + kSecond * second, more = !first;
+            const int slots = min(kBlockK, depth - kb * kBlockK + 15) / 16;  // what is behind the reduction is zeros
+            ok = parts::wait(full(st), (it / kStages) & 1, p.status, 93, abort_flag);
+            if (ok && first && chunks > 1) ok = parts::wait(acc_empty + 8 * second, ((chunks >> 1) - 1) & 1, p.status, 94, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const uint32_t dst = base + st * M::stage;
-            if (rank == 0) mbar_expect_tx(full(st), M::stage << PAIR);
-            load_3d<PAIR>(dst, map_a, kb * kBlockK, t.row + rank * kTileM, 0, full(st));
-            const int col = t.col + rank * M::right;
-            if (phase == kApply) {
-#pragma unroll
-              for (int j = 0; j < M::right / 64; ++j) load_3d<PAIR>(dst + (4 + 2 * j) * kBox, map_b, col + j * 64, kb * kBlockK, 0, full(st));
+            tc_fence_after();
+            if (wide) {  // a, a_lo: the first and last parts, or the middle and first
+              if (z == 0)
+                for (int k = 0; k < slots; ++k) mma_one<PAIR>(d, a + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
+              for (int k = 0; k < slots; ++k) {
+                mma_one<PAIR>(d, a + k * slot_a, b_lo + k * slot_b, desc_hi, idesc, more | (uint32_t)(k > 0));
+                mma_one<PAIR>(d, a_lo + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
+              }
+              if (z == 0)
+                for (int k = 0; k < slots; ++k) mma_one<PAIR>(d, a_lo + k * slot_a, b_lo + k * slot_b, desc_hi, idesc, 1);
+            } else if (slots == kBlockK / 16) {
+              mma_block<PAIR>(d, a, a_lo, b, b_lo, slot_b, desc_hi, idesc, more);
             } else {
-              load_3d<PAIR>(dst + 4 * kBox, map_b, kb * kBlockK, col, 0, full(st));
+              for (int k = 0; k < slots; ++k) {
+                mma_one<PAIR>(d, a + k * slot_a, b_lo + k * slot_b, desc_hi, idesc, more | (uint32_t)(k > 0));
+                mma_one<PAIR>(d, a_lo + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
+              }
+              for (int k = 0; k < slots; ++k) mma_one<PAIR>(d, a + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
+            }
+            kb += z == 0;
+            z = z == 0 && wide;
+            commit<PAIR>(empty(st));
+            if (last) {
+              commit<PAIR>(acc_full + 8 * second);
+              ++chunks;
             }
           }
         }
       }
-      if (!ok) asm volatile("red.relaxed.gpu.global.or.b32 [%0], %1;" ::"l"(p.arrived), "r"(kGaveUp) : "memory");
-      // what the MMA warp tells of the last stages has arrived before the CTA may leave, and copies that nobody has waited for have landed
-      for (int i = it > kStages ? it - kStages : 0; ok && i < it; ++i) ok = parts::wait(empty(i % kStages), (i / kStages) & 1, p.status, 99, abort_flag);
-      if (!ok && rank == 0)
-        for (int i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait(full(i % kStages), (i / kStages) & 1, p.status, 92);
-    }
-  } else if (warp == M::mma) {
-    if (rank == 0) {
-    // Descriptors as in parts_common.cuh: groups of 8 rows (of 8 K) 1024 bytes apart, 128-byte swizzle; where the columns lie side by side instead of
-    // the reduction, groups of 64 columns, both planes of them, 2 * kBox apart.
-    constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    constexpr uint32_t lbo = (2 * kBox >> 4) << 16, slot_a = 32 >> 4;  // mma_block has the latter as 2
-    int it = 0;
-    uint32_t chunks = 0;
-    for (int product = 0; product < 3 * p.steps && ok; ++product) {
-      const int phase = product % 3, items = p.items[phase];
-      const uint32_t slot_b = phase == kApply ? 2048 >> 4 : 32 >> 4;
-      const uint32_t idesc = (1u << 4) | (uint32_t)(phase == kApply) << 16 | (uint32_t)(M::rows >> 4) << 24 | (uint32_t)(W >> 3) << 17;
-      for (int i = unit; i < items && ok; i += units) {
-        const Tile t = tile_of<W, PAIR>(p, phase, i);
-        const int depth = phase == kGram ? p.item[t.q].n : p.item[t.q].m, chunk = chunk_of<W>(depth);
-        for (int kb = t.k0, in_chunk = 0; kb < t.k1 && ok; ++kb, ++it) {
-          const int st = it % kStages;
-          const bool first = in_chunk == 0, last = ++in_chunk == chunk || kb + 1 == t.k1;
-          if (last) in_chunk = 0;
-          const uint32_t a = ((base + st * M::stage) >> 4 & 0x3FFF) | lbo, b = ((base + st * M::stage + 4 * kBox) >> 4 & 0x3FFF) | lbo;
-          const uint32_t a_lo = a + (2 * kBox >> 4), b_lo = b + ((phase == kApply ? 1 : M::right / 64) * kBox >> 4), second = chunks & 1;
-          const uint32_t d = tmem + kSecond * second, more = !first;
-          const int slots = min(kBlockK, depth - kb * kBlockK + 15) / 16;  // what is behind the reduction is zeros
-          ok = parts::wait(full(st), (it / kStages) & 1, p.status, 93, abort_flag);
-          if (ok && first && chunks > 1) ok = parts::wait(acc_empty + 8 * second, ((chunks >> 1) - 1) & 1, p.status, 94, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          if (slots == kBlockK / 16) {
-            mma_block<PAIR>(d, a, a_lo, b, b_lo, slot_b, desc_hi, idesc, more);
-          } else {
-            for (int k = 0; k < slots; ++k) {
-              mma_one<PAIR>(d, a + k * slot_a, b_lo + k * slot_b, desc_hi, idesc, more | (uint32_t)(k > 0));
-              mma_one<PAIR>(d, a_lo + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
-            }
-            for (int k = 0; k < slots; ++k) mma_one<PAIR>(d, a + k * slot_a, b + k * slot_b, desc_hi, idesc, 1);
-          }
-          commit<PAIR>(empty(st));
-          if (last) {
-            commit<PAIR>(acc_full + 8 * second);
-            ++chunks;
-          }
+      }
+    } else {
+      Accumulators acc;
+      acc.rank = rank;
+      acc.quad = warp & 3;
+      acc.group = warp >> 2;
+      acc.lane = lane;
+      acc.sums = tmem + ((uint32_t)(acc.quad * 32) << 16) + acc.group * M::cols;
+      acc.full = acc_full;
+      acc.empty = acc_empty;
+      acc.chunks = 0;
+      acc.ok = true;
+      acc.wide = wide_ones;
+      acc.abort = abort_flag;
+      acc.drawn = reinterpret_cast<volatile int*>(tmem_slot + 2);
+      acc.slab = reinterpret_cast<float*>(smem + M::slab);
+      for (int step = 0; step < p.steps; ++step) {
+  #pragma unroll 1
+        for (int phase = 0; phase < 3; ++phase) {
+          const int product = 3 * step + phase;
+          if (product > 0 && acc.ok) acc.ok = __all_sync(0xffffffffu, parts::wait(go, (product - 1) & 1, p.status, 98, abort_flag));
+          if (phase == kGram) finish_tiles<kGram, W, PAIR, WIDE_ONES>(p, acc, step);
+          else if (phase == kSquare) finish_tiles<kSquare, W, PAIR, WIDE_ONES>(p, acc, step);
+          else if (step + 1 < p.steps) finish_tiles<kApply, W, PAIR, WIDE_ONES>(p, acc, step);
+          else finish_tiles<kResult, W, PAIR, WIDE_ONES>(p, acc, step);
+          if (product + 1 == 3 * p.steps) break;
+          asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
+          if (threadIdx.x == 0 && !*abort_flag) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.arrived) : "memory");
         }
       }
     }
-    }
-  } else {
-    Accumulators acc;
-    acc.rank = rank;
-    acc.quad = warp & 3;
-    acc.group = warp >> 2;
-    acc.lane = lane;
-    acc.sums = tmem + ((uint32_t)(acc.quad * 32) << 16) + acc.group * M::cols;
-    acc.full = acc_full;
-    acc.empty = acc_empty;
-    acc.chunks = 0;
-    acc.ok = true;
-    acc.abort = abort_flag;
-    acc.drawn = reinterpret_cast<volatile int*>(tmem_slot + 2);
-    acc.slab = reinterpret_cast<float*>(smem + M::slab);
-    for (int step = 0; step < p.steps; ++step) {
-#pragma unroll 1
-      for (int phase = 0; phase < 3; ++phase) {
-        const int product = 3 * step + phase;
-        if (product > 0 && acc.ok) acc.ok = __all_sync(0xffffffffu, parts::wait(go, (product - 1) & 1, p.status, 98, abort_flag));
-        if (phase == kGram) finish_tiles<kGram, W, PAIR>(p, acc, step & 1);
-        else if (phase == kSquare) finish_tiles<kSquare, W, PAIR>(p, acc, step & 1);
-        else if (step + 1 < p.steps) finish_tiles<kApply, W, PAIR>(p, acc, step & 1);
-        else finish_tiles<kResult, W, PAIR>(p, acc, step & 1);
-        if (product + 1 == 3 * p.steps) break;
-        asm volatile("bar.sync 1, %0;" ::"n"(M::warps * 32) : "memory");
-        if (threadIdx.x == 0 && !*abort_flag) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.arrived) : "memory");
-      }
-    }
-  }
+  };
+  if (wide_ones == 0) run(std::false_type());
+  else run(std::true_type());
   tc_fence_before();
   if (PAIR) cg::this_cluster().sync();  // neither leaves while the other still uses its memory
   else __syncthreads();
@@ -798,12 +893,15 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
   }
 }
 
-// X as parts: the update divided by its norm, its shorter side first.  Tiles of 64 x 64, turned in shared memory where that is the columns.
+// X as parts, of either kind: the update divided by its norm, its shorter side first.  Tiles of 64 x 64, turned in shared memory where that is
+// the columns.  And the sums of the squares of X's rows and columns, in units of 2^-60 (the sum of all is 1), so that the order in which tiles are
+// added does not matter; one that is not zero counts one unit at least.
 struct Parts {
   Update u[kGroup];
   int64_t rows[kGroup], cols[kGroup];
   const double* sums[kGroup];
-  uint16_t* x[kGroup];
+  uint16_t *x[kGroup], *x_wide[kGroup];
+  unsigned long long* sizes[kGroup];  // of the rows, then the columns of X
   int ldx[kGroup];
   unsigned first[kGroup + 1];  // tiles of the matrices before
   int count;
@@ -845,24 +943,64 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
     else tile[row + 4 * k][lane] = w;
   }
   __syncthreads();
-  const int64_t m = tall ? cols : rows, y0 = tall ? c0 : r0, x0 = tall ? r0 : c0, ld = p.ldx[q], plane = m * ld;
-  const int pair = threadIdx.x & 31, y = threadIdx.x >> 5, high = x0 + 2 * pair < ld ? (int)min((int64_t)64, m - y0) - y : 0;  // the padding of a row: zeros
-  uint16_t* o = p.x[q] + (y0 + y) * ld + x0 + 2 * pair;
+  const int64_t m = tall ? cols : rows, n = tall ? rows : cols, y0 = tall ? c0 : r0, x0 = tall ? r0 : c0, ld = p.ldx[q], plane = m * ld;
+  {  // four threads a row, four a column; what is outside is zeros, or NaN if the norm is
+    const int line = threadIdx.x >> 2, k0 = (threadIdx.x & 3) * 16;
+    float of_row = 0.f, of_col = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k, o += 8 * ld) {
+    for (int k = 0; k < 16; ++k) {
+      const float a = tile[line][k0 + k], b = tile[k0 + k][line];
+      of_row += a != 0.f ? fmaxf(a * a, 0x1p-100f) : 0.f;
+      of_col += b != 0.f ? fmaxf(b * b, 0x1p-100f) : 0.f;
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      of_row += __shfl_xor_sync(0xffffffffu, of_row, o);
+      of_col += __shfl_xor_sync(0xffffffffu, of_col, o);
+    }
+    if (k0 == 0 && y0 + line < m && of_row > 0.f) atomicAdd(p.sizes[q] + y0 + line, max(1ull, (unsigned long long)(of_row * 0x1p60f)));
+    if (k0 == 0 && x0 + line < n && of_col > 0.f) atomicAdd(p.sizes[q] + m + x0 + line, max(1ull, (unsigned long long)(of_col * 0x1p60f)));
+  }
+  const int pair = threadIdx.x & 31, y = threadIdx.x >> 5, high = x0 + 2 * pair < ld ? (int)min((int64_t)64, m - y0) - y : 0;  // the padding of a row: zeros
+  const int64_t at_o = (y0 + y) * ld + x0 + 2 * pair;
+  uint16_t *o = p.x[q] + at_o, *o_wide = p.x_wide[q] + at_o;
+#pragma unroll
+  for (int k = 0; k < 8; ++k, o += 8 * ld, o_wide += 8 * ld) {
     if (8 * k >= high) break;
-    uint32_t hi, lo;
-    split2(tile[y + 8 * k][2 * pair], tile[y + 8 * k][2 * pair + 1], hi, lo);
+    const float a = tile[y + 8 * k][2 * pair], b = tile[y + 8 * k][2 * pair + 1];
+    uint32_t hi, lo, w[kPlanes];
+    split2(a, b, kScale, hi, lo);
     *reinterpret_cast<uint32_t*>(o) = hi;
     *reinterpret_cast<uint32_t*>(o + plane) = lo;
+    split3(a, b, w);
+#pragma unroll
+    for (int i = 0; i < kPlanes; ++i) *reinterpret_cast<uint32_t*>(o_wide + i * plane) = w[i];
   }
 }
+// Which matrices have a row or column that is too faint for two parts (see above).
+struct Faint {
+  const unsigned long long* sizes[kGroup];
+  int64_t m[kGroup], n[kGroup];
+  unsigned* wide;
+};
+__global__ void __launch_bounds__(kThreads) faint_kernel(const __grid_constant__ Faint p) {
+  RT_PDL_ENTRY();
+  const int q = blockIdx.y;
+  const unsigned long long* sizes = p.sizes[q];
+  const int64_t m = p.m[q], n = p.n[q];
+  bool faint = false;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < m + n; i += (int64_t)gridDim.x * kThreads) {
+    const unsigned long long v = __ldg(sizes + i);
+    faint |= v != 0 && v < (unsigned long long)(i < m ? n : m) << 20;  // (sqrt(k) 2^-20)^2 2^60
+  }
+  if (__syncthreads_or(faint) && threadIdx.x == 0) atomicOr(p.wide, 1u << q);
+}
 
-// [2 planes][rows][cols] halves, rows ld apart, boxes of 64 columns and `height` rows of both planes, zeros outside.
+// [kPlanes][rows][cols] 16-bit values, rows ld apart, boxes of 64 columns and `height` rows of two planes, zeros outside.
 bool map_planes(CUtensorMap* map, uint16_t* t, int64_t cols, int64_t rows, int64_t ld, int height) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 2}, strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(ld * rows) * 2};
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, kPlanes}, strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(ld * rows) * 2};
   const cuuint32_t box[3] = {64, (cuuint32_t)height, 2}, one[3] = {1, 1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, t, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -959,10 +1097,11 @@ rt_status launch_products(rt_ctx* ctx, const Product& p) {
 rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int steps, bool* unavailable) {
   Product p{};
   Parts x{};
+  Faint f{};
   p.count = x.count = count;
   p.status = ctx->device_status;
   p.polls = ctx->sequence_polls;
-  size_t halves = 0, at[kGroup];
+  size_t halves = 0, sizes = 0, at[kGroup];
   for (int q = 0; q < count; ++q) {
     Item& i = p.item[q];
     i.m = (int)std::min(list[q].rows, list[q].cols);
@@ -970,7 +1109,8 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     i.ldx = (i.n + 7) / 8 * 8;
     i.ldm = (i.m + 7) / 8 * 8;
     at[q] = halves;
-    halves += ((size_t)4 * i.m * i.ldx + (size_t)4 * i.m * i.ldm + 63) / 64 * 64;
+    halves += ((size_t)2 * kPlanes * i.m * (i.ldx + i.ldm) + 63) / 64 * 64;
+    sizes += (size_t)(i.m + i.n);
     i.out = list[q].out;
     i.tall = list[q].rows > list[q].cols;
     i.update = list[q].update;
@@ -1001,17 +1141,21 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     tickets = std::max(tickets, (size_t)first_ticket * 2);
   }
   RtScratch work(ctx);
-  rt_status st = work.alloc(sizeof(uint16_t) * halves + sizeof(float) * partials + sizeof(double) * kNormBlocks * count + sizeof(unsigned) * (tickets + 1));
+  rt_status st = work.alloc(sizeof(uint16_t) * halves + sizeof(float) * partials + sizeof(double) * kNormBlocks * count + sizeof(unsigned long long) * (sizes + 1) +
+                            sizeof(unsigned) * (tickets + 1));
   if (st != RT_OK) return st;
   p.sums = reinterpret_cast<float*>(work.as<uint16_t>() + halves);
   double* squares = reinterpret_cast<double*>(p.sums + partials);
-  p.tickets = reinterpret_cast<unsigned*>(squares + (size_t)kNormBlocks * count);
+  unsigned long long *const zeros = reinterpret_cast<unsigned long long*>(squares + (size_t)kNormBlocks * count), *size = zeros + 1;
+  p.wide = reinterpret_cast<unsigned*>(zeros);
+  p.tickets = reinterpret_cast<unsigned*>(zeros + 1 + sizes);
   p.arrived = p.tickets + tickets;
   unsigned tiles = 0;
+  int longest = 0;
   const int right = plan.width == 64 ? 64 : plan.width / 2;  // columns that a CTA brings in
   for (int q = 0; q < count; ++q) {
     Item& i = p.item[q];
-    const size_t of_x = (size_t)2 * i.m * i.ldx, of_g = (size_t)2 * i.m * i.ldm;
+    const size_t of_x = (size_t)kPlanes * i.m * i.ldx, of_g = (size_t)kPlanes * i.m * i.ldm;
     i.x[0] = work.as<uint16_t>() + at[q];
     i.x[1] = i.x[0] + of_x;
     i.g = i.x[1] + of_x;
@@ -1030,6 +1174,12 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     x.cols[q] = list[q].cols;
     x.sums[q] = squares + (size_t)kNormBlocks * q;
     x.x[q] = i.x[0];
+    x.x_wide[q] = i.x[1];
+    f.sizes[q] = x.sizes[q] = size;
+    size += i.m + i.n;
+    f.m[q] = i.m;
+    f.n[q] = i.n;
+    longest = std::max(longest, i.m + i.n);
     x.ldx[q] = i.ldx;
     x.first[q] = tiles;
     tiles += (unsigned)((list[q].rows + 63) / 64 * ((list[q].cols + 63) / 64));
@@ -1037,8 +1187,11 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
   x.first[count] = tiles;
   x.tickets = p.tickets;
   x.tickets_end = (unsigned)tickets + 1;  // and the count of the blocks
-  if ((st = launch_squares(ctx, list, count, squares)) != RT_OK) return st;
+  f.wide = reinterpret_cast<unsigned*>(zeros);
+  if ((st = launch_squares(ctx, list, count, squares, zeros, (int64_t)sizes + 1)) != RT_OK) return st;
   rt_launch(ctx, parts_kernel, tiles, kThreads, 0, x);
+  RT_LAUNCHED(ctx);
+  rt_launch(ctx, faint_kernel, dim3(std::min((longest + kThreads - 1) / kThreads, 64), count), kThreads, 0, f);
   RT_LAUNCHED(ctx);
   return plan.width == 256 ? launch_products<256, true>(ctx, p) : (plan.width == 128 ? launch_products<128, true>(ctx, p) : launch_products<64, false>(ctx, p));
 }

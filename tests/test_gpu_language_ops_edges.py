@@ -1,4 +1,5 @@
-"""The operators of language models at their edges, beside test_gpu_language_ops.py: waits that run out, infinite values."""
+"""The operators of language models at their edges, beside test_gpu_language_ops.py: waits that run out, infinite values,
+rows and columns of a matrix that are faint against the others, matrices that are small as a whole."""
 import ctypes as C
 
 import numpy as np
@@ -111,3 +112,118 @@ def test_a_wait_of_muon_that_runs_out(shapes):
     for x, d in zip(host, p):
         as_near_as_fp32(d.numpy(), steps_on_gpu(x, torch.float64), steps_on_gpu(x, torch.float32))
     api.close()
+
+
+# ---- Muon: rows by themselves ---------------------------------------------------------------------------------------------------------
+
+
+def rows_as_near_as_fp32(got, want, plain, x):
+    """Every row against its own size.  X = D X' with rows of X' of norm 1: G = D G' D and the polynomial likewise, so that what a step adds up
+    for row i has the factor d_i, and all of as_near_as_fp32's 301 U of one step hold for row i against its own norm, r_i.  Matrices whose
+    faint rows and columns are not below sqrt(n) 2^-20 are held to 2^-40 (half a step of what is below 2^-22) instead: 2^-20 of a row, 16 U; their G and
+    polynomial, too, (4.775 * 2^-40 + 2^-39) |X| in every element of a row, at most as much again.  So one step is off by 333 U of the row that it
+    begins with; that is the last step's by a norm that is at most 1 / 0.63 of the result's, since a step multiplies singular values below 1.21 by
+    between 0.63 and 3.4445; steps before grow as in fp32: three times what the same steps are off there."""
+    norm = np.linalg.norm
+    rows = norm(x.astype(np.float64), axis=1) / (norm(x.astype(np.float64)) + 1e-7)
+    off = norm(got.astype(np.float64) - want, axis=1)
+    allowed = 3 * norm(plain - want, axis=1) + 333 * ref.U * np.maximum(rows, norm(want, axis=1) / 0.63)
+    worst = np.argmax(off / np.maximum(allowed, 1e-300))
+    assert np.all(off <= allowed), (worst, off[worst], allowed[worst], rows[worst])
+
+
+def check(capi, xs, steps=5):
+    """Each matrix's rows and columns; all of the list in one call."""
+    import torch
+
+    d, outs = [capi.to_device(x) for x in xs], [capi.empty(x.shape) for x in xs]
+    capi.call("orthogonalize_list", len(xs), pointers(d), capi.i64([x.shape[0] for x in xs]), capi.i64([x.shape[1] for x in xs]), steps, pointers(outs))
+    for x, o in zip(xs, outs):
+        if x.size > 1 << 20 and steps == 5:
+            want, plain = steps_on_gpu(x, torch.float64), steps_on_gpu(x, torch.float32)
+        else:
+            want, plain = ref.orthogonalize(x, steps), ref.orthogonalize(x, steps, np.float32)
+        got = o.numpy()
+        rows_as_near_as_fp32(got, want, plain, x)
+        rows_as_near_as_fp32(got.T, want.T, plain.T, x.T)
+
+
+FACTORS = 2.0 ** -np.array([0, 4, 8, 12, 14, 16, 18, 20, 22, 24, 28, 32, 40, 60])
+
+
+def graded(r, n, most=0):
+    """Factors of n rows, in blocks, down to 2^-most; most rows have none."""
+    f = np.ones(n)
+    steps = FACTORS[FACTORS >= 2.0**-most]
+    for k, block in enumerate(np.array_split(r.permutation(n)[: max(1, n // 2)], len(steps))):
+        f[block] = steps[k]
+    return f
+
+
+@pytest.mark.parametrize("most", [8, 16, 20, 24, 60])
+@pytest.mark.parametrize("side", ["rows", "columns", "both"])
+def test_faint_rows_and_columns(capi, side, most):
+    r = rng(61 + most)
+    xs = []
+    for shape in ((784, 128), (128, 784), (300, 260), (40, 700), (65, 64)):
+        x = r.standard_normal(shape)
+        if side != "columns":
+            x = x * graded(r, shape[0], most)[:, None]
+        if side != "rows":
+            x = x * graded(r, shape[1], most)
+        xs.append(x.astype(np.float32))
+    check(capi, xs)
+    check(capi, xs, 1)
+
+
+def test_faint_rows_of_large_matrices(capi):
+    """Tiles of pairs of CTAs; in one list with matrices that have no faint rows."""
+    r = rng(62)
+    shape = (1501, 1603)
+    plain = matrix(r, shape)
+    check(capi, [(r.standard_normal(shape) * graded(r, shape[0], 60)[:, None]).astype(np.float32), plain])
+    check(capi, [(r.standard_normal(s) * graded(r, s[1], 32)).astype(np.float32) for s in [(1290, 1803)] * 2] + [matrix(r, (1803, 1290))] * 4)
+
+
+def test_faint_copies_of_rows(capi):
+    """Rows that are another row over again, but for a small factor, do not grow with the small singular values."""
+    r = rng(63)
+    x = r.standard_normal((200, 300))
+    x[100:150] = x[:50] * FACTORS[np.arange(50) % len(FACTORS), None]
+    check(capi, [x.astype(np.float32), x.T.astype(np.float32)])
+
+
+@pytest.mark.parametrize("value", [1e-7, 1e-12, 1e-20, 1e-30])
+def test_small_matrices_are_not_lost(capi, value):
+    """The norm is not much more than what is added to it, or less: the result is small, and has a value."""
+    r = rng(64)
+    check(capi, [(value * r.standard_normal(s) / s[0]).astype(np.float32) for s in ((40, 30), (150, 200), (700, 512))])
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("shape", [(1, 6), (6, 1), (65, 3), (30, 700), (1290, 1803)])
+def test_matrices_with_a_special_value(capi, shape, value):
+    """All of the result is NaN; that of the list's other matrix is what it is by itself."""
+    r = rng(70)
+    x, y = matrix(r, shape), matrix(r, (33, 130))
+    x[0, -1] = value
+    d, outs = [capi.to_device(a) for a in (x, y)], [capi.empty(a.shape) for a in (x, y)]
+    capi.call("orthogonalize_list", 2, pointers(d), capi.i64([shape[0], 33]), capi.i64([shape[1], 130]), 5, pointers(outs))
+    assert np.isnan(outs[0].numpy()).all()
+    as_near_as_fp32(outs[1].numpy(), ref.orthogonalize(y), ref.orthogonalize(y, 5, np.float32))
+
+
+def test_sparse_rows(capi):
+    """Rows of zeros stay zeros; rows with a single element, down to small ones; all of it the same in every run."""
+    r = rng(65)
+    x = r.standard_normal((260, 333)).astype(np.float32)
+    x[::3] = 0
+    for k, i in enumerate(range(0, 240, 6)):
+        x[i, (7 * i) % 333] = 2.0 ** -(k + 1)
+    check(capi, [x, np.ascontiguousarray(x.T)])
+    d, outs = capi.to_device(x), [capi.empty(x.shape) for _ in range(3)]
+    for o in outs:
+        capi.call("orthogonalize_list", 1, pointers([d]), capi.i64([260]), capi.i64([333]), 5, pointers([o]))
+    got = [o.numpy() for o in outs]
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+    assert np.all(got[0][3::6] == 0)
