@@ -492,8 +492,10 @@ rt_status rt_optimizer_step_multi(rt_ctx* ctx, int kind, int n_tensors, float* c
  * [rows, cols] that rows are multiplied with (x * W).  Per matrix: m = momentum * m + s * g with s = grad_scale; u = m, or s * g + momentum * m
  * with nesterov; p = (1 - lr * weight_decay) * p - lr * sqrt(max(1, cols / rows)) * O(u).  O(u): `steps` (0 .. 64; five are usual) times
  * X = (a I + b G + c G^2) X, G = X X^T on the shorter side, from X = u / (|u| + 1e-7), with a, b, c = 3.4445, -4.7750, 2.0315.  Products
- * to about fp32's precision, every row and column against its own size however faint it is beside the others.  All matrices of the list are worked on together: the same call gives the same bits, another list may change the
- * last of them.  Shorter sides up to 65536, longer ones below 2^24.  Parameters and momenta must overlap neither one another nor the gradients.
+ * to about fp32's precision, every row and column against its own size however faint it is beside the others.  All matrices of
+ * the list are worked on together: the same call gives the same bits, another list may change the last of them.  Shorter sides up to 65536,
+ * longer ones below 2^24.  Parameters and momenta must overlap neither one another nor the gradients.
+ * A call that finds no room has changed nothing; without tensor cores, where each product looks for room, it has updated the matrices before.
  * Blocks wait for one another between the products (rt_lstm_sequence_polls): if a wait runs out, which the next synchronising call says, momenta
  * have been updated and parameters have not, or a part of them if it was in the last product. */
 rt_status rt_muon_step_multi(rt_ctx* ctx, int n_tensors, float* const* params, const float* const* grads, float* const* momenta, const int64_t* rows,

@@ -45,22 +45,26 @@ struct Update {
   float mu, scale;
   int nesterov;
 };
+__device__ __forceinline__ float momentum_at(const Update& u, int64_t i) { return u.mu * u.m[i] + u.scale * __ldg(u.g + i); }
+// From the old momentum.
 __device__ __forceinline__ float update_at(const Update& u, int64_t i) {
   if (!u.g) return __ldg(u.x + i);
-  return u.nesterov ? u.scale * __ldg(u.g + i) + u.mu * u.m[i] : u.m[i];
+  const float m = momentum_at(u, i);
+  return u.nesterov ? u.scale * __ldg(u.g + i) + u.mu * m : m;
 }
-// The new momentum, and the sum of the squares of the update, block by block in 64 bits: squares of large fp32 values have no room in 32.  A
+// The new momentum, if it is to be written by now, and the sum of the squares of the update, block by block in 64 bits: squares of large fp32 values have no room in 32.  A
 // matrix has kNormBlocks blocks.  Bound by memory: 4096 x 4096 takes 17 us (236 with one value at a time in 128 blocks).
 constexpr int kGroup = 12;  // matrices of a launch
 struct Squares {
   Update u[kGroup];
   int64_t n[kGroup];
+  int write;
   double* sums;  // [matrix][block]
   unsigned long long* zero;  // what later launches begin with zeros
   int64_t zeros;
 };
 template <bool VEC>
-__device__ __forceinline__ double sum_of_squares(const Update& u, int64_t n) {
+__device__ __forceinline__ double sum_of_squares(const Update& u, int64_t n, bool write) {
   constexpr int kAhead = 4, V = VEC ? 4 : 1;
   double sum = 0.0;
   const int64_t step = (int64_t)kNormBlocks * kThreads * V;
@@ -97,7 +101,7 @@ __device__ __forceinline__ double sum_of_squares(const Update& u, int64_t n) {
         }
         sum += v * v;
       }
-      if (u.g && i < n) {
+      if (write && i < n) {
         if (VEC) *reinterpret_cast<float4*>(u.m + i) = make_float4(m[k][0], m[k][V / 4], m[k][V / 2], m[k][V - 1]);
         else u.m[i] = m[k][0];
       }
@@ -113,7 +117,8 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
   const Update u = p.u[q];
   const int64_t n = p.n[q];
   const bool vec = n % 4 == 0 && (((uintptr_t)u.x | (uintptr_t)u.g | (uintptr_t)u.m) & 15) == 0;
-  double sum = vec ? sum_of_squares<true>(u, n) : sum_of_squares<false>(u, n);
+  const bool write = p.write && u.g;
+  double sum = vec ? sum_of_squares<true>(u, n, write) : sum_of_squares<false>(u, n, write);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = sum;
@@ -149,14 +154,15 @@ __global__ void __launch_bounds__(kThreads) polynomial_kernel(const float* __res
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < m * m; i += (int64_t)gridDim.x * kThreads)
     s[i] = kB * __ldg(g + i) + kC * s[i] + (i / m == i % m ? kA : 0.f);
 }
-// out = keep * out - step * x, or out = x
+// out = keep * out - step * x, or out = x; and the new momentum
 __global__ void __launch_bounds__(kThreads) apply_kernel(const float* __restrict__ x, int64_t rows, int64_t cols, float* __restrict__ out, int update, float keep,
-                                                         float step) {
+                                                         float step, const Update u) {
   RT_PDL_ENTRY();
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * kThreads) {
     const int64_t r = i / cols, c = i - r * cols;
     const float o = __ldg(x + (rows > cols ? c * rows + r : i));
     out[i] = update ? keep * out[i] - step * o : o;
+    if (u.g) u.m[i] = momentum_at(u, i);
   }
 }
 
@@ -168,12 +174,13 @@ struct Matrix {
   float keep, step;
 };
 
-rt_status launch_squares(rt_ctx* ctx, const Matrix* list, int count, double* sums, unsigned long long* zero = nullptr, int64_t zeros = 0) {
+rt_status launch_squares(rt_ctx* ctx, const Matrix* list, int count, int write, double* sums, unsigned long long* zero = nullptr, int64_t zeros = 0) {
   Squares p{};
   for (int q = 0; q < count; ++q) {
     p.u[q] = list[q].u;
     p.n[q] = list[q].rows * list[q].cols;
   }
+  p.write = write;
   p.sums = sums;
   p.zero = zero;
   p.zeros = zeros;
@@ -1028,7 +1035,7 @@ struct Cost {
   double block, rest, shared, share;
 };
 constexpr Cost kCosts[3] = {{1140, 7600, 3600, 500}, {1400, 12600, 7000, 950}, {2230, 23900, 12200, 3900}};
-Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
+Plan plan_products(const int (&fit)[3], int count, const Item* items) {
   Plan best{};
   double least = 1e300;
   for (int width = 64; width <= 256; width *= 2) {
@@ -1036,7 +1043,8 @@ Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
     p.width = width;
     double sum = 0;
     const Cost& cost = kCosts[width / 128];
-    const int units = width == 64 ? ctx->sm_count : ctx->sm_count / 2;
+    const int units = fit[width / 128];
+    if (units == 0) continue;
     for (int phase = 0; phase < 3; ++phase) {
       double least_here = 1e300;
       int deepest = 1;
@@ -1070,17 +1078,13 @@ Plan plan_products(const rt_ctx* ctx, int count, const Item* items) {
   return best;
 }
 template <int W, bool PAIR>
-rt_status launch_products(rt_ctx* ctx, const Product& p) {
+cudaLaunchConfig_t config(const rt_ctx* ctx, unsigned blocks, cudaLaunchAttribute (&at)[2]) {
   using M = Layout<W, PAIR>;
-  static RtDeviceOnce once;
-  RT_CUDA(ctx, once([] { return cudaFuncSetAttribute(newton_schulz_kernel<W, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)M::bytes); }));
-  const int items = std::max(p.items[0], std::max(p.items[1], p.items[2])), units = ctx->sm_count >> PAIR;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = (unsigned)std::min(items, units) << PAIR;
+  cfg.gridDim = blocks;
   cfg.blockDim = M::threads;
   cfg.dynamicSmemBytes = M::bytes;
   cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeCooperative;
   at[0].val.cooperative = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
@@ -1088,29 +1092,70 @@ rt_status launch_products(rt_ctx* ctx, const Product& p) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = PAIR ? 2 : 1;
+  return cfg;
+}
+// How many CTAs or pairs the device runs at once, which is what waits for one another; asked once.
+template <int W, bool PAIR>
+rt_status units_of(rt_ctx* ctx, int* units) {
+  if (*units >= 0) return RT_OK;
+  using M = Layout<W, PAIR>;
+  static RtDeviceOnce once;
+  RT_CUDA(ctx, once([] { return cudaFuncSetAttribute(newton_schulz_kernel<W, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)M::bytes); }));
+  int n = 0;
+  if (PAIR) {
+    cudaLaunchAttribute at[2];
+    cudaLaunchConfig_t cfg = config<W, PAIR>(ctx, 2, at);
+    cfg.attrs = at + 1;
+    cfg.numAttrs = 1;
+    RT_CUDA(ctx, cudaOccupancyMaxActiveClusters(&n, newton_schulz_kernel<W, PAIR>, &cfg));
+  } else {
+    RT_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, newton_schulz_kernel<W, PAIR>, M::threads, M::bytes));
+    n *= ctx->sm_count;
+  }
+  *units = std::min(n, ctx->sm_count >> PAIR);
+  return RT_OK;
+}
+template <int W, bool PAIR>
+rt_status launch_products(rt_ctx* ctx, const Product& p) {
+  const int items = std::max(p.items[0], std::max(p.items[1], p.items[2]));
+  cudaLaunchAttribute at[2];
+  const cudaLaunchConfig_t cfg = config<W, PAIR>(ctx, (unsigned)std::min(items, ctx->muon_units[W / 128]) << PAIR, at);
   RT_CUDA(ctx, cudaLaunchKernelEx(&cfg, newton_schulz_kernel<W, PAIR>, p));
   RT_LAUNCHED(ctx);
   return RT_OK;
 }
 
-// Up to kGroup matrices together.
-rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int steps, bool* unavailable) {
+// Up to kGroup matrices together.  What may fail comes before the first launch: sizes, room and tensor maps.
+struct Group {
   Product p{};
   Parts x{};
   Faint f{};
-  p.count = x.count = count;
+  Plan plan{};
+  const Matrix* list = nullptr;
+  int count = 0;
+  size_t halves = 0, sizes = 0, partials = 0, tickets = 0, at[kGroup] = {};
+  double* squares = nullptr;
+  size_t bytes() const {
+    return sizeof(uint16_t) * halves + sizeof(float) * partials + sizeof(double) * kNormBlocks * count + sizeof(unsigned long long) * (sizes + 1) +
+           sizeof(unsigned) * (tickets + 1);
+  }
+};
+void lay_out(const rt_ctx* ctx, const Matrix* list, int count, int steps, Group* group) {
+  Product& p = group->p;
+  group->list = list;
+  group->count = p.count = group->x.count = count;
   p.status = ctx->device_status;
   p.polls = ctx->sequence_polls;
-  size_t halves = 0, sizes = 0, at[kGroup];
+  p.steps = steps;
   for (int q = 0; q < count; ++q) {
     Item& i = p.item[q];
     i.m = (int)std::min(list[q].rows, list[q].cols);
     i.n = (int)std::max(list[q].rows, list[q].cols);
     i.ldx = (i.n + 7) / 8 * 8;
     i.ldm = (i.m + 7) / 8 * 8;
-    at[q] = halves;
-    halves += ((size_t)2 * kPlanes * i.m * (i.ldx + i.ldm) + 63) / 64 * 64;
-    sizes += (size_t)(i.m + i.n);
+    group->at[q] = group->halves;
+    group->halves += ((size_t)2 * kPlanes * i.m * (i.ldx + i.ldm) + 63) / 64 * 64;
+    group->sizes += (size_t)(i.m + i.n);
     i.out = list[q].out;
     i.tall = list[q].rows > list[q].cols;
     i.update = list[q].update;
@@ -1118,9 +1163,7 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     i.keep = list[q].keep;
     i.step = list[q].step;
   }
-  p.steps = steps;
-  const Plan plan = plan_products(ctx, count, p.item);
-  size_t partials = 0, tickets = 0;
+  const Plan& plan = group->plan = plan_products(ctx->muon_units, count, p.item);
   for (int phase = 0; phase < 3; ++phase) {
     int items = 0, first_part = 0, first_ticket = 0;
     for (int q = 0; q < count; ++q) {
@@ -1137,26 +1180,28 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
       }
     }
     p.items[phase] = items;
-    partials = std::max(partials, (size_t)first_part * plan.width * rows_of_tile(plan.width));
-    tickets = std::max(tickets, (size_t)first_ticket * 2);
+    group->partials = std::max(group->partials, (size_t)first_part * plan.width * rows_of_tile(plan.width));
+    group->tickets = std::max(group->tickets, (size_t)first_ticket * 2);
   }
-  RtScratch work(ctx);
-  rt_status st = work.alloc(sizeof(uint16_t) * halves + sizeof(float) * partials + sizeof(double) * kNormBlocks * count + sizeof(unsigned long long) * (sizes + 1) +
-                            sizeof(unsigned) * (tickets + 1));
-  if (st != RT_OK) return st;
-  p.sums = reinterpret_cast<float*>(work.as<uint16_t>() + halves);
-  double* squares = reinterpret_cast<double*>(p.sums + partials);
-  unsigned long long *const zeros = reinterpret_cast<unsigned long long*>(squares + (size_t)kNormBlocks * count), *size = zeros + 1;
-  p.wide = reinterpret_cast<unsigned*>(zeros);
-  p.tickets = reinterpret_cast<unsigned*>(zeros + 1 + sizes);
-  p.arrived = p.tickets + tickets;
+}
+// False if a tensor map cannot be had.
+bool place(Group* group, void* memory) {
+  Product& p = group->p;
+  Parts& x = group->x;
+  uint16_t* halves = static_cast<uint16_t*>(memory);
+  p.sums = reinterpret_cast<float*>(halves + group->halves);
+  group->squares = reinterpret_cast<double*>(p.sums + group->partials);
+  unsigned long long *const zeros = reinterpret_cast<unsigned long long*>(group->squares + (size_t)kNormBlocks * group->count), *size = zeros + 1;
+  p.wide = group->f.wide = reinterpret_cast<unsigned*>(zeros);
+  p.tickets = reinterpret_cast<unsigned*>(zeros + 1 + group->sizes);
+  p.arrived = p.tickets + group->tickets;
   unsigned tiles = 0;
-  int longest = 0;
-  const int right = plan.width == 64 ? 64 : plan.width / 2;  // columns that a CTA brings in
-  for (int q = 0; q < count; ++q) {
+  const int right = group->plan.width == 64 ? 64 : group->plan.width / 2;  // columns that a CTA brings in
+  for (int q = 0; q < group->count; ++q) {
+    const Matrix& of = group->list[q];
     Item& i = p.item[q];
     const size_t of_x = (size_t)kPlanes * i.m * i.ldx, of_g = (size_t)kPlanes * i.m * i.ldm;
-    i.x[0] = work.as<uint16_t>() + at[q];
+    i.x[0] = halves + group->at[q];
     i.x[1] = i.x[0] + of_x;
     i.g = i.x[1] + of_x;
     i.s = i.g + of_g;
@@ -1165,46 +1210,51 @@ rt_status orthogonalize_together(rt_ctx* ctx, const Matrix* list, int count, int
     for (int k = 0; k < 2; ++k)
       mapped = mapped && map_planes(&p.x_left[k][q], i.x[k], i.n, i.m, i.ldx, kTileM) && map_planes(&p.x_right[k][q], i.x[k], i.n, i.m, i.ldx, right) &&
                map_planes(&p.x_apply[k][q], i.x[k], i.n, i.m, i.ldx, 64);
-    if (!mapped) {
-      *unavailable = true;
-      return RT_OK;
-    }
-    x.u[q] = list[q].u;
-    x.rows[q] = list[q].rows;
-    x.cols[q] = list[q].cols;
-    x.sums[q] = squares + (size_t)kNormBlocks * q;
+    if (!mapped) return false;
+    x.u[q] = of.u;
+    x.rows[q] = of.rows;
+    x.cols[q] = of.cols;
+    x.sums[q] = group->squares + (size_t)kNormBlocks * q;
     x.x[q] = i.x[0];
     x.x_wide[q] = i.x[1];
-    f.sizes[q] = x.sizes[q] = size;
+    group->f.sizes[q] = x.sizes[q] = size;
     size += i.m + i.n;
-    f.m[q] = i.m;
-    f.n[q] = i.n;
-    longest = std::max(longest, i.m + i.n);
+    group->f.m[q] = i.m;
+    group->f.n[q] = i.n;
     x.ldx[q] = i.ldx;
     x.first[q] = tiles;
-    tiles += (unsigned)((list[q].rows + 63) / 64 * ((list[q].cols + 63) / 64));
+    tiles += (unsigned)((of.rows + 63) / 64 * ((of.cols + 63) / 64));
   }
-  x.first[count] = tiles;
+  x.first[group->count] = tiles;
   x.tickets = p.tickets;
-  x.tickets_end = (unsigned)tickets + 1;  // and the count of the blocks
-  f.wide = reinterpret_cast<unsigned*>(zeros);
-  if ((st = launch_squares(ctx, list, count, squares, zeros, (int64_t)sizes + 1)) != RT_OK) return st;
-  rt_launch(ctx, parts_kernel, tiles, kThreads, 0, x);
+  x.tickets_end = (unsigned)group->tickets + 1;  // and the count of the blocks
+  return true;
+}
+rt_status launch(rt_ctx* ctx, const Group& group) {
+  rt_status st = launch_squares(ctx, group.list, group.count, 1, group.squares, group.x.sizes[0] - 1, (int64_t)group.sizes + 1);
+  if (st != RT_OK) return st;
+  rt_launch(ctx, parts_kernel, group.x.first[group.count], kThreads, 0, group.x);
   RT_LAUNCHED(ctx);
-  rt_launch(ctx, faint_kernel, dim3(std::min((longest + kThreads - 1) / kThreads, 64), count), kThreads, 0, f);
+  int longest = 0;
+  for (int q = 0; q < group.count; ++q) longest = std::max(longest, group.p.item[q].m + group.p.item[q].n);
+  rt_launch(ctx, faint_kernel, dim3(std::min((longest + kThreads - 1) / kThreads, 64), group.count), kThreads, 0, group.f);
   RT_LAUNCHED(ctx);
-  return plan.width == 256 ? launch_products<256, true>(ctx, p) : (plan.width == 128 ? launch_products<128, true>(ctx, p) : launch_products<64, false>(ctx, p));
+  const int width = group.plan.width;
+  return width == 256 ? launch_products<256, true>(ctx, group.p) : (width == 128 ? launch_products<128, true>(ctx, group.p) : launch_products<64, false>(ctx, group.p));
 }
 
 // ---- by the framework's other products: without tensor cores, or with no steps ------------------------------------------------------------
-rt_status orthogonalize(rt_ctx* ctx, const Matrix& q, int steps) {
+size_t bytes_otherwise(const Matrix& q) {
+  const size_t m = (size_t)std::min(q.rows, q.cols), n = (size_t)std::max(q.rows, q.cols);
+  return sizeof(double) * kNormBlocks + sizeof(float) * (2 * m * n + 2 * m * m);
+}
+// The momentum is written with the result: a product may not find room for itself.
+rt_status orthogonalize(rt_ctx* ctx, const Matrix& q, int steps, void* memory) {
   const int64_t m = std::min(q.rows, q.cols), n = std::max(q.rows, q.cols), all = m * n;
-  RtScratch work(ctx);
-  rt_status st = work.alloc(sizeof(double) * kNormBlocks + sizeof(float) * (size_t)(2 * all + 2 * m * m));
-  if (st != RT_OK) return st;
-  double* sums = work.as<double>();
+  double* sums = static_cast<double*>(memory);
   float *x = reinterpret_cast<float*>(sums + kNormBlocks), *y = x + all, *g = y + all, *s = g + m * m;
-  if ((st = launch_squares(ctx, &q, 1, sums)) != RT_OK) return st;
+  rt_status st = launch_squares(ctx, &q, 1, 0, sums);
+  if (st != RT_OK) return st;
   rt_launch(ctx, normalise_kernel, rt_grid_for(ctx, all, kThreads), kThreads, 0, q.u, q.rows, q.cols, sums, x);
   RT_LAUNCHED(ctx);
   for (int k = 0; k < steps; ++k) {
@@ -1215,19 +1265,45 @@ rt_status orthogonalize(rt_ctx* ctx, const Matrix& q, int steps) {
     if ((st = rt_gemm(ctx, 0, 0, m, n, m, s, m, x, n, y, n, 0)) != RT_OK) return st;
     std::swap(x, y);
   }
-  rt_launch(ctx, apply_kernel, rt_grid_for(ctx, all, kThreads), kThreads, 0, x, q.rows, q.cols, q.out, q.update, q.keep, q.step);
+  rt_launch(ctx, apply_kernel, rt_grid_for(ctx, all, kThreads), kThreads, 0, x, q.rows, q.cols, q.out, q.update, q.keep, q.step, q.u);
   RT_LAUNCHED(ctx);
   return RT_OK;
 }
+// Everything is ready before the first launch, which changes momenta.
 rt_status orthogonalize_all(rt_ctx* ctx, const std::vector<Matrix>& list, int steps) {
+  if (list.empty()) return RT_OK;
   rt_status st = RT_OK;
-  for (size_t first = 0; first < list.size(); first += kGroup) {
-    const int count = (int)std::min<size_t>(kGroup, list.size() - first);
-    bool otherwise = steps == 0 || !ctx->use_tensor_cores;
-    if (!otherwise && (st = orthogonalize_together(ctx, &list[first], count, steps, &otherwise)) != RT_OK) return st;
-    for (int q = 0; otherwise && q < count; ++q)
-      if ((st = orthogonalize(ctx, list[first + q], steps)) != RT_OK) return st;
+  bool together = steps > 0 && ctx->use_tensor_cores;
+  int(&units)[3] = ctx->muon_units;
+  if (together) {
+    if ((st = units_of<64, false>(ctx, &units[0])) != RT_OK || (st = units_of<128, true>(ctx, &units[1])) != RT_OK ||
+        (st = units_of<256, true>(ctx, &units[2])) != RT_OK)
+      return st;
+    together = units[0] || units[1] || units[2];
   }
+  RtScratch work(ctx);
+  std::vector<Group> groups;
+  if (together) {
+    groups.resize((list.size() + kGroup - 1) / kGroup);
+    size_t bytes = 0;
+    for (size_t k = 0; k < groups.size(); ++k) {
+      lay_out(ctx, &list[k * kGroup], (int)std::min<size_t>(kGroup, list.size() - k * kGroup), steps, &groups[k]);
+      bytes = std::max(bytes, groups[k].bytes());
+    }
+    if ((st = work.alloc(bytes)) != RT_OK) return st;
+    for (Group& g : groups) together = together && place(&g, work.ptr);
+  }
+  if (together) {
+    for (const Group& g : groups)
+      if ((st = launch(ctx, g)) != RT_OK) return st;
+    return RT_OK;
+  }
+  RtScratch other(ctx);
+  size_t bytes = 0;
+  for (const Matrix& q : list) bytes = std::max(bytes, bytes_otherwise(q));
+  if ((st = other.alloc(bytes)) != RT_OK) return st;
+  for (const Matrix& q : list)
+    if ((st = orthogonalize(ctx, q, steps, other.ptr)) != RT_OK) return st;
   return RT_OK;
 }
 

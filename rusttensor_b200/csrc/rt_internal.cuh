@@ -67,6 +67,7 @@ struct rt_ctx {
   bool use_tma_weight_grad = true;
   // How many clusters of 2 .. 16 CTAs of the medium products' kernel this device holds at a time ([1]: set once that is known).
   int ts_clusters[17] = {};
+  int muon_units[3] = {-1, -1, -1};  // CTAs or pairs of them of k_muon.cu's products that this device runs at once, by width of the tiles
   uint32_t sequence_polls = 1u << 21;  // looks at what another block has not sent yet (k_lstm_seq.cu, k_gated_scan.cu, k_muon.cu)
   // NCCL (loaded at run time on first use)
   void* nccl_comm = nullptr;

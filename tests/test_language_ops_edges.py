@@ -1,0 +1,15 @@
+"""The operators of language models on the CPU, at their edges: tests/host/muon_checks.cpp over stubs of the CUDA runtime."""
+import os
+import subprocess
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def test_muon_changes_nothing_before_it_is_known_that_it_can(tmp_path):
+    obj, exe = str(tmp_path / "muon.o"), str(tmp_path / "muon_checks")
+    subprocess.run([os.environ.get("NVCC", "nvcc"), "-gencode", "arch=compute_100a,code=compute_100a", "-std=c++17", "-c",
+                    os.path.join(os.path.dirname(HERE), "rusttensor_b200", "csrc", "k_muon.cu"), "-o", obj], check=True)
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-I/usr/local/cuda/include", "-o", exe,
+                    os.path.join(HERE, "host", "muon_checks.cpp"), obj], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
