@@ -693,12 +693,12 @@ rt_status rt_embedding_backward(rt_ctx* ctx, const float* g, const int32_t* ids,
   if (st != RT_OK) return st;
   if (rows == 0 || cols == 0) return RT_OK;
   RT_CHECK_PTR(ctx, dtable);
+  RtOnDevice here(ctx);
   if (n == 0) return accumulate ? RT_OK : rt_fill(ctx, dtable, 0.f, rows * cols);
   RT_CHECK_PTR(ctx, g);
   RT_CHECK_PTR(ctx, ids);
   if (rt_overlap(dtable, 4 * rows * cols, g, 4 * n * cols) || rt_overlap(dtable, 4 * rows * cols, ids, 4 * n))
     RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_embedding_backward: dtable overlaps what is read");
-  RtOnDevice here(ctx);
   int bits = 1;  // of the largest key, which is `rows`
   while (bits < 32 && (uint64_t)rows >> bits) ++bits;
   const bool vec = cols % 4 == 0 && rt_aligned16(g) && rt_aligned16(dtable);

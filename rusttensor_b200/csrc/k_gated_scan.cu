@@ -610,6 +610,7 @@ rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, in
   if (st == RT_OK) st = check_sizes(ctx, "rt_gated_scan_backward", steps, batch, hidden, ld < ldd ? ldd : ld);
   if (st != RT_OK) return st;
   if (batch == 0 || hidden == 0) return RT_OK;
+  RtOnDevice here(ctx);
   if (steps == 0) return dh0 ? rt_fill(ctx, dh0, 0.f, batch * hidden) : RT_OK;
   RT_CHECK_PTR(ctx, f);
   RT_CHECK_PTR(ctx, v);
@@ -625,7 +626,6 @@ rt_status rt_gated_scan_backward(rt_ctx* ctx, const float* f, const float* v, in
       if (meet(w, r)) RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_gated_scan_backward: a result overlaps what is read");
   if (meet(written[0], written[1]) || meet(written[0], written[2]) || meet(written[1], written[2]))
     RT_FAIL(ctx, RT_ERR_INVALID_OPERATION, "rt_gated_scan_backward: results overlap");
-  RtOnDevice here(ctx);
   ScanArgs s{};
   s.f = f;
   s.v = v;

@@ -1,4 +1,5 @@
-"""The operators of language models on the CPU, at their edges: tests/host/muon_checks.cpp over stubs of the CUDA runtime."""
+"""The operators of language models on the CPU, at their edges: tests/host/muon_checks.cpp and language_device_checks.cpp, over stubs of the
+CUDA runtime."""
 import os
 import subprocess
 
@@ -11,5 +12,17 @@ def test_muon_changes_nothing_before_it_is_known_that_it_can(tmp_path):
                     os.path.join(os.path.dirname(HERE), "rusttensor_b200", "csrc", "k_muon.cu"), "-o", obj], check=True)
     subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-I/usr/local/cuda/include", "-o", exe,
                     os.path.join(HERE, "host", "muon_checks.cpp"), obj], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_launches_are_on_the_context_s_device(tmp_path):
+    csrc, exe = os.path.join(os.path.dirname(HERE), "rusttensor_b200", "csrc"), str(tmp_path / "language_device_checks")
+    objs = [str(tmp_path / (name + ".o")) for name in ("k_embedding", "k_gated_scan")]
+    for obj in objs:
+        subprocess.run([os.environ.get("NVCC", "nvcc"), "-gencode", "arch=compute_100a,code=compute_100a", "-std=c++17", "-c",
+                        os.path.join(csrc, os.path.basename(obj).replace(".o", ".cu")), "-o", obj], check=True)
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-I/usr/local/cuda/include", "-o", exe,
+                    os.path.join(HERE, "host", "language_device_checks.cpp")] + objs, check=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
