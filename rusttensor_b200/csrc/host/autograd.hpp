@@ -1087,12 +1087,14 @@ Tensor<B> fused_lstm_sequence(const Tensor<B>& x, const Tensor<B>& w, const Tens
 
 // ---- ops that the reference does not have ---------------------------------------------------------------------------------
 // scale * table[ids], a row for every entry of ids, which holds whole numbers like the results of argmax: [ids' shape..., cols].  What is no
-// row's number is padding: zeros, and no gradient.  A backend without the kernels multiplies one-hot rows with the table, as the
+// row's number is padding: zeros, and no gradient.  Tables have 2^24 rows at most: a float above holds even numbers only, and an odd one would be
+// another token's.  A backend without the kernels multiplies one-hot rows with the table, as the
 // reference's char-LSTM example does (examples/lstm_char_rnn_cpu.rs).
 template <class B>
 Tensor<B> embedding(const Tensor<B>& table, const Tensor<B>& ids, float scale) {
   const Shape ts = table.shape(), is = ids.shape();
   if (ts.size() != 2) throw Error::invalid_op("embedding expects a table [rows, cols]");
+  if (ts[0] > (size_t)1 << 24) throw Error::invalid_op("embedding takes tables of 2^24 rows at most");
   Shape os = is;
   os.push_back(ts[1]);
   if constexpr (!HasFusedForward<B>::value) {

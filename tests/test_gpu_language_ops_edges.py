@@ -1,5 +1,6 @@
 """The operators of language models at their edges, beside test_gpu_language_ops.py: waits that run out, infinite values,
-rows and columns of a matrix that are faint against the others, matrices that are small as a whole."""
+rows and columns of a matrix that are faint against the others, matrices that are small as a whole, the
+largest table."""
 import ctypes as C
 
 import numpy as np
@@ -8,6 +9,7 @@ import pytest
 import language_ref as ref
 import rusttensor_b200
 from helpers import rng
+from rusttensor_b200.frontend import EngineError
 from test_gpu_language_ops import as_near_as_fp32, f32, i64, matrix, pointers, steps_on_gpu
 
 pytestmark = pytest.mark.gpu
@@ -227,3 +229,21 @@ def test_sparse_rows(capi):
     got = [o.numpy() for o in outs]
     assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
     assert np.all(got[0][3::6] == 0)
+
+
+# ---- embeddings ---------------------------------------------------------------------------------------------------------------------------
+
+
+def test_the_largest_table_of_the_engine(gpu_engine):
+    """2^24 rows: every number is one of its own, the next one is padding as it is rounded; a row more is refused."""
+    e, rows = gpu_engine, 2**24
+    table = np.arange(rows, dtype=np.float32).reshape(rows, 1)
+    t = e.tensor(table, requires_grad=True)
+    ids = np.array([rows - 1, rows - 2, 0, rows, rows + 1])
+    out = e.ops.embedding(t, e.tensor(ids.astype(np.float32)))
+    assert out.numpy().ravel().tolist() == [rows - 1, rows - 2, 0, 0, 0]
+    e.ops.sum(out).backward()
+    assert np.flatnonzero(t.grad.numpy()).tolist() == [0, rows - 2, rows - 1]
+    with pytest.raises(EngineError) as ei:
+        e.ops.embedding(e.tensor(np.zeros((rows + 1, 1), np.float32)), e.tensor(ids.astype(np.float32)))
+    assert ei.value.kind == "InvalidOperation"

@@ -3,6 +3,11 @@ CUDA runtime."""
 import os
 import subprocess
 
+import numpy as np
+import pytest
+
+from rusttensor_b200.frontend import EngineError
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
@@ -26,3 +31,14 @@ def test_launches_are_on_the_context_s_device(tmp_path):
                     os.path.join(HERE, "host", "language_device_checks.cpp")] + objs, check=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_tables_whose_numbers_floats_do_not_hold_are_refused(oracle_engine):
+    """Token numbers are held as floats: 2^24 + 1 would be 2^24."""
+    e = oracle_engine
+    with pytest.raises(EngineError) as ei:
+        e.ops.embedding(e.tensor(np.zeros((2**24 + 1, 1), np.float32)), e.tensor(np.array([2**24])))
+    assert ei.value.kind == "InvalidOperation"
+    with pytest.raises(EngineError) as ei:  # and none of them is made into one-hot rows first
+        e.ops.embedding(e.tensor(np.zeros((2**24 + 1, 1), np.float32)), e.tensor(np.zeros(0)))
+    assert ei.value.kind == "InvalidOperation"
