@@ -60,11 +60,11 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const float* __rest
   }
 }
 
-// Whole numbers held as floats, as the engine holds them; everything else (fractions, NaN, beyond int32) becomes -1.
-__global__ void __launch_bounds__(kThreads) token_ids_kernel(const float* __restrict__ x, int64_t n, int32_t* __restrict__ ids) {
+// Whole numbers held as floats, as the engine holds them; everything else (fractions, NaN, beyond int32) becomes -1.  In place, too: no read-only loads.
+__global__ void __launch_bounds__(kThreads) token_ids_kernel(const float* x, int64_t n, int32_t* ids) {
   RT_PDL_ENTRY();
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-    const float v = __ldg(x + i);
+    const float v = x[i];
     ids[i] = v >= 0.f && v < 2147483648.f && v == truncf(v) ? (int32_t)v : -1;
   }
 }

@@ -247,3 +247,17 @@ def test_the_largest_table_of_the_engine(gpu_engine):
     with pytest.raises(EngineError) as ei:
         e.ops.embedding(e.tensor(np.zeros((rows + 1, 1), np.float32)), e.tensor(ids.astype(np.float32)))
     assert ei.value.kind == "InvalidOperation"
+
+
+@pytest.mark.parametrize("n", [1, 1000, 3000001])
+def test_token_ids_in_place(capi, n):
+    """Numbers and what is none, in the place that they are read from: the same as elsewhere."""
+    r = rng(71)
+    x = r.integers(-3, 2**24, n).astype(np.float32)
+    x[::7] += 0.5
+    x[::11] = np.nan
+    d, out = capi.to_device(x), capi.empty((n,))
+    capi.call("token_ids", d.ptr, i64(n), out.ptr)
+    capi.call("token_ids", d.ptr, i64(n), d.ptr)
+    want = np.where((x >= 0) & (x == np.trunc(x)), np.nan_to_num(x), -1).astype(np.int64)
+    assert np.array_equal(out.numpy().view(np.int32), want) and np.array_equal(d.numpy().view(np.int32), want)
