@@ -1464,10 +1464,11 @@ struct B200Backend {
     const bool given = o.inputs.size() > 1;
     const float *p = gates.ptr(), *p0 = given ? o.inputs[1].data().ptr() : nullptr, *pg = g.ptr(), *states = h.ptr();
     const bool written = h.buf->escaped && !lazy::capturing();  // perhaps, since
-    lazy::Block again(ctx(), written ? (size_t)(rows * H) : 1);
+    std::optional<lazy::Block> again;
     if (written) {
-      check(rt_gated_scan(ctx(), p, p + H, 2 * H, p0, (int64_t)steps, batch, H, again.ptr));
-      states = again.ptr;
+      again.emplace(ctx(), (size_t)(rows * H));
+      check(rt_gated_scan(ctx(), p, p + H, 2 * H, p0, (int64_t)steps, batch, H, again->ptr));
+      states = again->ptr;
     }
     const bool to_start = given && o.inputs[1].requires_grad();
     std::vector<Storage> out{alloc(gates.shape)};
