@@ -231,6 +231,31 @@ def test_sparse_rows(capi):
     assert np.all(got[0][3::6] == 0)
 
 
+def test_a_graph_goes_by_its_inputs(capi):
+    """Captured with matrices that have no faint rows, replayed with some that do and back: the bits of a call on the same inputs."""
+    r = rng(72)
+    shapes = [(300, 200), (1290, 1803)]
+    plain = [matrix(r, s) for s in shapes]
+    faint = [(x * graded(r, x.shape[0], 60)[:, None]).astype(np.float32) for x in plain]
+    d, outs = [capi.to_device(x) for x in plain], [capi.empty(s) for s in shapes]
+    args = (len(shapes), pointers(d), capi.i64([s[0] for s in shapes]), capi.i64([s[1] for s in shapes]), 5, pointers(outs))
+    fill = lambda xs: [capi.check(capi.lib.rt_memcpy_h2d(capi.ctx, t.ptr, x.ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes))) for x, t in zip(xs, d)]  # noqa: E731
+    want = []
+    for xs in (plain, faint, [plain[0], faint[1]]):
+        fill(xs)
+        capi.call("orthogonalize_list", *args)
+        want.append([o.numpy() for o in outs])
+    graph = C.c_void_p()
+    capi.call("graph_begin")
+    capi.call("orthogonalize_list", *args)
+    capi.call("graph_end", C.byref(graph))
+    for xs, w in zip((plain, faint, [plain[0], faint[1]], plain), want + want[:1]):
+        fill(xs)
+        capi.call("graph_launch", graph)
+        assert all(np.array_equal(o.numpy(), b) for o, b in zip(outs, w))
+    capi.call("graph_destroy", graph)
+
+
 # ---- embeddings ---------------------------------------------------------------------------------------------------------------------------
 
 
