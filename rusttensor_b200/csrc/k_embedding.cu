@@ -4,6 +4,9 @@
 //
 // A number outside the table is padding: zeros forward, no term backward.  The gradient adds the rows of one token in the order of their
 // positions, whatever runs when: the pairs (token, position) are sorted by token first, stably, and no sum is made with atomics.
+//
+// rt_gather_rows, the gather of a data set's rows, reads the same but neither scales nor has as many loads in flight: 32768 rows of 1024 of
+// 50000 take 33.5 us there and 29.7 here, 64 of 512 1.7 either way (replayed from a graph).
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -561,9 +564,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_runs_kernel(const Runs r) {
   }
 }
 // Few tokens, in one launch: a warp has a row of the table and 32 pieces of the columns, looks through all tokens and adds what is its row's.
-// 128 tokens, added to 1000 rows of 1024: 3.8 us, 10.1 sorted.  Tables of more than 65536 such units are left to the sort: 8000 rows of 1024,
-// which are 64000, take 5.7 and 9.6 us, 50000 rows, of which every warp has 80, 24 and 9.9.  All tokens the same is what bounds this: one row of
-// g after the other.
+// 128 tokens, added to 1000 rows of 1024: 5.6 us, 12.4 sorted.  Tables of more than 65536 such units are left to the sort: 8000 rows of 1024,
+// which are 64000, take 6.0 and 12.4 us, 16000 rows 9.8 and 12.4, 50000, of which every warp has 42 units, 25 and 12.8; written instead of added to
+// 8.8 and 14.2, 15.5 and 18.6, 44 and 35: they meet at some 20000.  (A unit is 128 columns, 32 where rows are not aligned.)  All tokens the same is what bounds this: one row
+// of g after the other.
 constexpr int kFew = 128;
 constexpr int64_t kFewUnits = 1 << 16;
 template <bool VEC, bool ACCUMULATE>

@@ -12,10 +12,12 @@
 // that it starts from and its timesteps are a multiply-add each.  Everything is read and written once; the loads of the next stretch
 // are in flight meanwhile, or those of other blocks.  What is added in which order depends on the sizes alone.
 //
-// Bound by memory, 12 bytes an element forward and 24 backward, and near that by the instructions (about 40 and 60 an element; 88 backward
-// with one column at a time).  Measured, in TB/s of those bytes: 128 timesteps of 64 x 512 11.7 us forward (4.3), 19.5 backward (5.2); 1000 of
-// 16 x 1000 38.3 (5.0); 65536 of 1 x 512 85 (4.8) and 166 (4.9); 30011 of 3 x 257 backward 131 (4.2).  A thread per column, which reads ahead
-// eight timesteps, takes 24 us for the first and 9.4 ms for the third; it remains for up to eight timesteps.
+// 12 bytes an element forward and 24 backward, in TB/s of those: 128 timesteps of 64 x 512 11.4 us forward (4.4), 19.7 backward (5.1); 1000 of 16 x 1000
+// in matrices of their own 38 (5.0); 65536 of 1 x 512 87 - 95 (4.2 - 4.6) and 166 (4.9); 30011 of 3 x 257 backward 136 - 141 (3.9 - 4.1).  Nothing is
+// saturated there: long sequences take half of the memory's rate and half of the issue slots (46 and 80 instructions an element, 103 backward with one
+// column at a time) with a quarter of the warps, so it is what a warp waits for that counts, its loads and the exchange.  A training batch
+// in a row, which the L2 cache holds, takes rounds: 1024 strips for 592 places are two, each with its first loads' latency.  A thread
+// per column, which reads ahead eight timesteps, takes 24 us for the first and 9.4 ms for the third; it remains for up to eight timesteps.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -44,7 +46,7 @@ struct ScanArgs {
   uint32_t polls;  // looks at what another block of the cluster has not sent yet
 };
 // sigmoid(f) and 1 - sigmoid(f), each to the last bits: the smaller one is not the difference of two near ones.  1 + e lies in [1, 2], where the
-// approximate reciprocal is within one unit of the last place and a division of its own is not needed.
+// approximate reciprocal is within one unit of the last place (a division: half of one).
 __device__ __forceinline__ void gate(float f, float& a, float& rest) {
   const float e = expf(-fabsf(f));
   float large;
