@@ -3,22 +3,25 @@
 //   m = mu m + s g      u = m, or s g + mu m (nesterov)      p = (1 - lr wd) p - lr sqrt(max(1, cols / rows)) O(u)
 //
 // O(u) comes from Newton-Schulz steps on X = u / (|u| + 1e-7): X <- (a I + b G + c G^2) X with G = X X^T, which takes every singular value x to
-// a x + b x^3 + c x^5, with 3.4445, -4.7750, 2.0315, the coefficients published with Muon (K. Jordan, 2024): five steps bring values between 0.002 and 1 to between 0.7 and
-// 1.2.  G is taken on the shorter side; a matrix with more rows than columns is transposed for the steps.
+// a x + b x^3 + c x^5, with 3.4445, -4.7750, 2.0315, the coefficients published with Muon (K. Jordan, 2024): five steps bring values between 0.002 and
+// 1 to between 0.7 and 1.2.  G is taken on the shorter side; a matrix with more rows than columns is transposed for the steps.
 //
 // A step is three products, each of which has to wait for the one before: G = X X^T and b G + c G^2, both symmetric, of which the lower half is
 // computed and written twice, and a X + (b G + c G^2) X.  Errors of early steps grow (small singular values by 3.4 a step), so the products
 // keep fp32's precision: an operand is held as two fp16 parts, hi = fp16(2^15 x) and lo = fp16(2^15 x - hi), 22 bits, and a product is three
 // tcgen05.mma of kind::f16: hi lo, lo hi and hi hi.  No element of X, G or the polynomial is beyond 1.21, 1.46 and 2.81 (bounds of their singular
 // values; the polynomial takes 2^14), so the scale is fixed.  Below 2^-18, where lo has fewer than 11 bits left, an element is off by
-// 2^-40 at most, which is 2^-20 of a row or column of k elements as long as its norm is sqrt(k) 2^-20 or more: rows whose norms differ by exp(N(0, 1)), as in
-// 4096 x 4096, stay above that.  Where a row or a column that is not zero lies below, the matrix is wide: its operands are three bf16 parts, 24
-// bits of fp32's range, and a product is six MMAs (all but the three smallest), so that every row and column is as near as in fp32 against its own
-// size: what a step adds up for one has that size as a factor.  (With two parts rows 2^-16 of the others were 9e-5 off and rows 2^-32 of them not updated
-// at all.)  Rows and columns shrink by no more than a factor of ten over all steps, so this is decided once.  A product's epilogue adds what
-// the formula adds and writes the parts that the next product reads, as they lie: X [m][n] is an operand with n as the reduction, and with
-// m, by tensor maps and MMA descriptors of either kind.  All matrices of a call go through every product together, and all products are one
-// cooperative launch, whose blocks wait for one another between two products (15 launches for five steps were 4 us each besides the work).
+// 2^-40 at most, of G and the polynomial together by 2^-37.2 in its share of the result: that is 2^-19 of a row or column of k elements as long as its
+// norm is sqrt(max(k, 64)) 2^-21 or more.  Rows whose norms differ by exp(N(0, 1)) stay above that up to some 10000 x 10000.  Where a row or a
+// column that is not zero lies below, the matrix is wide: its operands are three bf16 parts, 24 bits of fp32's range, and a product is six MMAs
+// (all but the three smallest), so that every row and column is as near as in fp32 against its own size: what a step adds up for one has that
+// size as a factor.  (With two parts alone, at 2^12, rows 2^-16 of the others were 9e-5 off and rows 2^-32 of them not updated at all.)  Rows
+// and columns shrink by no more than a third over all steps (singular values up to 1 end above 0.68), so this is decided once.
+//
+// A product's epilogue adds what the formula adds and writes the parts that the next product reads, as they lie: X [m][n] is an operand with n as
+// the reduction, and with m, by tensor maps and MMA descriptors of either kind.  All matrices of a call go through every product together, and all
+// products are one cooperative launch, whose blocks wait for one another between two products (15 launches for five steps were 4 us each
+// besides the work).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -901,9 +904,14 @@ __global__ void __launch_bounds__(Layout<W, PAIR>::threads, 1) newton_schulz_ker
   }
 }
 
+__device__ __forceinline__ unsigned long long faint_below(int64_t elements) { return (unsigned long long)max(elements, (int64_t)64) << 18; }  // (sqrt(k) 2^-21)^2 2^60
+__device__ __forceinline__ void add_size(unsigned long long* to, float sum, int64_t elements) {
+  if (sum > 0.f && __ldcg(to) < faint_below(elements)) atomicAdd(to, max(1ull, (unsigned long long)(sum * 0x1p60f)));
+}
 // X as parts, of either kind: the update divided by its norm, its shorter side first.  Tiles of 64 x 64, turned in shared memory where that is
 // the columns.  And the sums of the squares of X's rows and columns, in units of 2^-60 (the sum of all is 1), so that the order in which tiles are
-// added does not matter; one that is not zero counts one unit at least.
+// added does not matter; one that is not zero counts one unit at least, and one that is known not to be faint is left as it is (adding on and on to few
+// rows: 64 x 500000 took 0.1 ms more).
 struct Parts {
   Update u[kGroup];
   int64_t rows[kGroup], cols[kGroup];
@@ -966,8 +974,8 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const __grid_constant__
       of_row += __shfl_xor_sync(0xffffffffu, of_row, o);
       of_col += __shfl_xor_sync(0xffffffffu, of_col, o);
     }
-    if (k0 == 0 && y0 + line < m && of_row > 0.f) atomicAdd(p.sizes[q] + y0 + line, max(1ull, (unsigned long long)(of_row * 0x1p60f)));
-    if (k0 == 0 && x0 + line < n && of_col > 0.f) atomicAdd(p.sizes[q] + m + x0 + line, max(1ull, (unsigned long long)(of_col * 0x1p60f)));
+    if (k0 == 0 && y0 + line < m) add_size(p.sizes[q] + y0 + line, of_row, n);
+    if (k0 == 0 && x0 + line < n) add_size(p.sizes[q] + m + x0 + line, of_col, m);
   }
   const int pair = threadIdx.x & 31, y = threadIdx.x >> 5, high = x0 + 2 * pair < ld ? (int)min((int64_t)64, m - y0) - y : 0;  // the padding of a row: zeros
   const int64_t at_o = (y0 + y) * ld + x0 + 2 * pair;
@@ -999,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads) faint_kernel(const __grid_constant__
   bool faint = false;
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < m + n; i += (int64_t)gridDim.x * kThreads) {
     const unsigned long long v = __ldg(sizes + i);
-    faint |= v != 0 && v < (unsigned long long)(i < m ? n : m) << 20;  // (sqrt(k) 2^-20)^2 2^60
+    faint |= v != 0 && v < faint_below(i < m ? n : m);
   }
   if (__syncthreads_or(faint) && threadIdx.x == 0) atomicOr(p.wide, 1u << q);
 }
@@ -1238,7 +1246,7 @@ rt_status launch(rt_ctx* ctx, const Group& group) {
   RT_LAUNCHED(ctx);
   int longest = 0;
   for (int q = 0; q < group.count; ++q) longest = std::max(longest, group.p.item[q].m + group.p.item[q].n);
-  rt_launch(ctx, faint_kernel, dim3(std::min((longest + kThreads - 1) / kThreads, 64), group.count), kThreads, 0, group.f);
+  rt_launch(ctx, faint_kernel, dim3(rt_grid_for(ctx, longest, kThreads), group.count), kThreads, 0, group.f);
   RT_LAUNCHED(ctx);
   const int width = group.plan.width;
   return width == 256 ? launch_products<256, true>(ctx, group.p) : (width == 128 ? launch_products<128, true>(ctx, group.p) : launch_products<64, false>(ctx, group.p));
@@ -1282,10 +1290,9 @@ rt_status orthogonalize_all(rt_ctx* ctx, const std::vector<Matrix>& list, int st
       return st;
     together = units[0] || units[1] || units[2];
   }
-  RtScratch work(ctx);
-  std::vector<Group> groups;
   if (together) {
-    groups.resize((list.size() + kGroup - 1) / kGroup);
+    RtScratch work(ctx);
+    std::vector<Group> groups((list.size() + kGroup - 1) / kGroup);
     size_t bytes = 0;
     for (size_t k = 0; k < groups.size(); ++k) {
       lay_out(ctx, &list[k * kGroup], (int)std::min<size_t>(kGroup, list.size() - k * kGroup), steps, &groups[k]);
@@ -1293,18 +1300,15 @@ rt_status orthogonalize_all(rt_ctx* ctx, const std::vector<Matrix>& list, int st
     }
     if ((st = work.alloc(bytes)) != RT_OK) return st;
     for (Group& g : groups) together = together && place(&g, work.ptr);
+    for (size_t k = 0; together && st == RT_OK && k < groups.size(); ++k) st = launch(ctx, groups[k]);
+    if (together) return st;
   }
-  if (together) {
-    for (const Group& g : groups)
-      if ((st = launch(ctx, g)) != RT_OK) return st;
-    return RT_OK;
-  }
-  RtScratch other(ctx);
+  RtScratch work(ctx);
   size_t bytes = 0;
   for (const Matrix& q : list) bytes = std::max(bytes, bytes_otherwise(q));
-  if ((st = other.alloc(bytes)) != RT_OK) return st;
+  if ((st = work.alloc(bytes)) != RT_OK) return st;
   for (const Matrix& q : list)
-    if ((st = orthogonalize(ctx, q, steps, other.ptr)) != RT_OK) return st;
+    if ((st = orthogonalize(ctx, q, steps, work.ptr)) != RT_OK) return st;
   return RT_OK;
 }
 
